@@ -43,6 +43,7 @@ typedef struct psi_pages psi_pages;
 typedef struct psi_table psi_table;
 typedef struct psi_gqa psi_gqa;
 typedef struct psi_id_allocator psi_id_allocator;
+typedef struct psi_linear psi_linear;
 
 typedef enum psi_status {
     PSI_OK = 0,
@@ -582,6 +583,71 @@ PSI_API int32_t psi_gqa_attend_static(int32_t device, void* cuda_stream, const p
                                       const uint32_t* token_indices, const uint32_t* cu_tokens, uint32_t num_reqs,
                                       uint32_t layer, const void* q, void* out, char* error, size_t error_len);
 
+/* ---- bounded sequence memory: no counterpart in the reference, whose caches only grow -------------------------------- */
+
+/* The attention weight that each cached key gathers from this step's queries, added to what it has:
+ *   weights[slot][kv head][j] += sum over the request's query tokens i and the group's q heads of
+ *                                softmax_j(scale q . k_j),     j in [0, token_index + i]
+ * for the prepared batch.  weights: device f32 [num_req_slots][Hkv][weights_stride], one buffer per layer, zeros for a request's
+ * first step; entries at and beyond a request's keys and the rows of other slots are not touched.  q: device [T][Hq][D] as given
+ * to psi_gqa_attend.  Enqueue after this step's K rows are in their pages.  A query row whose scores hold a NaN or have no
+ * finite maximum adds nothing.  Sums are f32 in a fixed order: the same call gives the same bits.
+ * 16-bit profiles whose head_dim is a multiple of eight run on the tensor cores and need q and the arena on 16-byte boundaries;
+ * every other profile of the component runs on the CUDA cores.  A batch that names a slot twice is refused.
+ * Scratch is allocated on the first call and grows with the batch (4 bytes per query row and key of the short runs, up to
+ * 2 GiB; without it the keys are read twice).  In a captured sequence (after psi_gqa_reserve_replay and one call outside the
+ * capture) weights_stride must hold the page table's whole row. */
+PSI_API int32_t psi_gqa_weigh_keys(psi_gqa* gqa, psi_pages* pages, psi_table* table, uint32_t layer, const void* q, float* weights,
+                                   uint64_t weights_stride);
+
+/* Cuts requests' caches of one layer down to their heaviest keys.  Per request r and KV head the keys [0, lengths[r]) of slot
+ * src_slots[r] leave, but for the last min(recent, keeps[r]) and the heaviest of the others by weights (the lower index
+ * where equal, NaN as the lightest), keeps[r] in all.  Their K and V rows move, in their old order, to tokens [0, keeps[r]) of
+ * slot dst_slots[r]: src_slots[r] itself, in place, or another slot whose page-table row names pages of its own (pages shared
+ * with other requests, as a prefix cache does, must not be cut in place).  Heads choose for themselves, so a token index no longer names
+ * one position: kept, device u32 [num_reqs][Hkv][kept_stride], receives the old indices in ascending order; entries beyond
+ * keeps[r] are left.  weights_out (same shape as weights, may be the same buffer) receives at [dst slot][head] the kept
+ * keys' weights and zeros for [keeps[r], lengths[r]).  Keys are cached after their rotation, so kept rows stay valid; the
+ * request's next token has token index keeps[r] in psi_gqa_prepare (and its true position wherever it is rotated).  Pages behind the last kept
+ * token are the caller's to free.  src_slots, dst_slots, lengths, keeps: host arrays, read before the call returns.  A slot
+ * may be a source once and a destination once, and a destination is no other request's source.  Works without a prepared
+ * batch; not inside a stream capture. */
+PSI_API int32_t psi_gqa_evict(psi_gqa* gqa, psi_pages* pages, psi_table* table, uint32_t layer, const uint32_t* src_slots,
+                              const uint32_t* dst_slots, const uint32_t* lengths, const uint32_t* keeps, uint32_t num_reqs,
+                              uint32_t recent, const float* weights, float* weights_out, uint64_t weights_stride, uint32_t* kept,
+                              uint64_t kept_stride);
+
+/* Linear attention with a decay for each head, for layers whose memory is a state instead of a cache: per value head, with
+ * lambda = exp(log_decay),
+ *   S_t = lambda S_{t-1} + k_t^T v_t,     o_t = scale q_t S_t,     S [key_dim][value_dim].
+ * q and k have num_k_heads heads; value head h reads k head h / (num_v_heads / num_k_heads).  key_dim and value_dim are
+ * multiples of 8 up to 256.  states: device f32 [num_req_slots][num_layers][Hv][key_dim][value_dim], the caller's,
+ * 16-byte aligned; it needs no clearing, since a request whose token_index is 0 starts from a zero state. */
+typedef struct psi_linear_config {
+    uint32_t num_k_heads;
+    uint32_t num_v_heads;
+    uint32_t key_dim;
+    uint32_t value_dim;
+    float scale;
+    uint32_t dtype; /* psi_dtype of q, k, v and out */
+    uint32_t num_req_slots;
+    uint32_t num_layers;
+    uint32_t max_tokens; /* flat token capacity of one step */
+} psi_linear_config;
+PSI_API int32_t psi_linear_create(psi_ctx* ctx, const psi_linear_config* config, psi_linear** out);
+PSI_API int32_t psi_linear_destroy(psi_linear* linear);
+/* log_decay: host array of num_v_heads values, finite and <= 0 (0, no decay, is the initial state). */
+PSI_API int32_t psi_linear_set_decay(psi_linear* linear, uint32_t layer, const float* log_decay);
+/* The step's batch, as for psi_gqa_prepare: host arrays, uploaded in one copy.  out_slots (NULL: req_slots) names the slot that
+ * receives each request's new state, so that a draft can be verified without losing the state before it; no two requests
+ * write one slot, and none writes a slot that another one reads.  A request without tokens changes nothing. */
+PSI_API int32_t psi_linear_prepare(psi_linear* linear, const uint32_t* req_slots, const uint32_t* out_slots,
+                                   const uint32_t* token_indices, const uint32_t* cu_tokens, uint32_t num_reqs);
+/* q, k device [T][Hk][key_dim], v, out device [T][Hv][value_dim]; out must not overlap the inputs.  Any number of tokens per
+ * request.  The same call gives the same bits.  May be captured: a replay takes the batch prepared last. */
+PSI_API int32_t psi_linear_attend(psi_linear* linear, uint32_t layer, float* states, const void* q, const void* k, const void* v,
+                                  void* out);
+
 /* Number of kernels this library has launched on the context since creation (for launch accounting). */
 PSI_API int32_t psi_ctx_launch_count(psi_ctx* ctx, uint64_t* out);
 
@@ -596,7 +662,10 @@ typedef enum psi_kernel_class {
     PSI_KERNEL_CLASS_COMBINE = 3,
     PSI_KERNEL_CLASS_GATHER = 4,
     PSI_KERNEL_CLASS_ATTEND_CHUNK = 5,
-    PSI_KERNEL_CLASS_NORM_ROPE_APPEND = 6
+    PSI_KERNEL_CLASS_NORM_ROPE_APPEND = 6,
+    PSI_KERNEL_CLASS_WEIGH = 7,
+    PSI_KERNEL_CLASS_EVICT = 8,
+    PSI_KERNEL_CLASS_LINEAR = 9
 } psi_kernel_class;
 PSI_API int32_t psi_ctx_enable_kernel_timing(psi_ctx* ctx, int32_t enable);
 PSI_API int32_t psi_ctx_kernel_timing(psi_ctx* ctx, uint32_t kernel_class, float* out_total_ms, uint64_t* out_launches);

@@ -8,5 +8,5 @@ from .binding import (  # noqa: F401
     PLAN_BALANCED, PLAN_REFERENCE, Context, GQA, GQAConfig, GQAPageTableLayout, KvExchange, GQAReplayShape, GQARequestPageTable,
     GQASplitKV, GQASplitKVVariant, NormRopeConfig, PageArena, PsiError, ReplayBucketPolicy, U32IDAllocator, ExecutorHibernationPlan, StateSnapshotReader, StateSnapshotWriter,
     SNAPSHOT_PAGE_ARENA, SNAPSHOT_MAIN_GQA_REQUEST_PAGE_TABLE, SNAPSHOT_MAIN_GDN_REQUEST_STATE_TABLE,
-    SNAPSHOT_MTP_GQA_REQUEST_PAGE_TABLE, SNAPSHOT_DSPARK_GQA_REQUEST_PAGE_TABLE, attend_static, library, library_path, rope_parameters,
+    SNAPSHOT_MTP_GQA_REQUEST_PAGE_TABLE, SNAPSHOT_DSPARK_GQA_REQUEST_PAGE_TABLE, LinearAttention, LinearConfig, attend_static, library, library_path, rope_parameters,
 )

@@ -697,9 +697,70 @@ class GQA:
         _check(library().psi_gqa_decode_step_host(self._h, pages._h, table._h, C.c_uint32(layer), _ptr(k_host),
                                                   _ptr(v_host), _ptr(q_host), _ptr(out_host)), self.ctx._h)
 
+    def weigh_keys(self, pages: PageArena, table: GQARequestPageTable, layer: int, q, weights, weights_stride: int):
+        """Add the attention weight that each cached key gathers from the prepared batch's queries to ``weights``
+        (f32 ``[num_req_slots][Hkv][weights_stride]``)."""
+        _check(library().psi_gqa_weigh_keys(self._h, pages._h, table._h, C.c_uint32(layer), _ptr(q), _ptr(weights),
+                                            C.c_uint64(weights_stride)), self.ctx._h)
+
+    def evict(self, pages: PageArena, table: GQARequestPageTable, layer: int, src_slots, dst_slots, lengths, keeps, recent: int,
+              weights, weights_out, weights_stride: int, kept, kept_stride: int):
+        """Cut caches down to the ``recent`` last and the heaviest other keys, ``keeps`` in all, per KV head; ``kept`` (u32
+        ``[requests][Hkv][kept_stride]``) receives their old indices, ``weights_out`` their weights."""
+        src, n = _u32_array(src_slots)
+        dst, n2 = _u32_array(dst_slots)
+        length, n3 = _u32_array(lengths)
+        keep, n4 = _u32_array(keeps)
+        if not n == n2 == n3 == n4:
+            raise PsiError(1, "src_slots, dst_slots, lengths and keeps lengths disagree")
+        _check(library().psi_gqa_evict(self._h, pages._h, table._h, C.c_uint32(layer), src, dst, length, keep, C.c_uint32(n),
+                                       C.c_uint32(recent), _ptr(weights), _ptr(weights_out), C.c_uint64(weights_stride),
+                                       _ptr(kept), C.c_uint64(kept_stride)), self.ctx._h)
+
     def page_gather(self, pages, table, req_slot, layer, tok_begin, tok_end, k_out, v_out):
         _check(library().psi_page_gather(self._h, pages._h, table._h, C.c_uint32(req_slot), C.c_uint32(layer),
                                          C.c_uint32(tok_begin), C.c_uint32(tok_end), _ptr(k_out), _ptr(v_out)),
+               self.ctx._h)
+
+
+class LinearConfig(C.Structure):
+    _fields_ = [("num_k_heads", C.c_uint32), ("num_v_heads", C.c_uint32), ("key_dim", C.c_uint32), ("value_dim", C.c_uint32),
+                ("scale", C.c_float), ("dtype", C.c_uint32), ("num_req_slots", C.c_uint32), ("num_layers", C.c_uint32),
+                ("max_tokens", C.c_uint32)]
+
+
+class LinearAttention:
+    """Linear attention with a decay for each head; ``states`` is f32 ``[num_req_slots][num_layers][Hv][key_dim][value_dim]``."""
+
+    def __init__(self, ctx: Context, config: LinearConfig):
+        self.ctx, self.config = ctx, config
+        self._h = C.c_void_p()
+        _check(library().psi_linear_create(ctx._h, C.byref(config), C.byref(self._h)), ctx._h)
+
+    def close(self):
+        if self._h:
+            library().psi_linear_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def set_decay(self, layer: int, log_decay):
+        """The logarithms of a layer's decays, one per value head, finite and not positive."""
+        values = [float(x) for x in log_decay]
+        if len(values) != self.config.num_v_heads:
+            raise PsiError(1, "log_decay must hold num_v_heads values")
+        _check(library().psi_linear_set_decay(self._h, C.c_uint32(layer), (C.c_float * len(values))(*values)), self.ctx._h)
+
+    def prepare(self, req_slots, token_indices, cu_tokens, out_slots=None):
+        """The step's batch; ``out_slots`` names the slots that receive the new states (``req_slots`` where omitted)."""
+        rs, n = _u32_array(req_slots)
+        ti, n2 = _u32_array(token_indices)
+        cu, n3 = _u32_array(cu_tokens)
+        outs, n4 = (None, n) if out_slots is None else _u32_array(out_slots)
+        if n != n2 or n3 != n + 1 or n4 != n:
+            raise PsiError(1, "req_slots, out_slots, token_indices and cu_tokens lengths disagree")
+        _check(library().psi_linear_prepare(self._h, rs, outs, ti, cu, C.c_uint32(n)), self.ctx._h)
+
+    def attend(self, layer: int, states, q, k, v, out):
+        _check(library().psi_linear_attend(self._h, C.c_uint32(layer), _ptr(states), _ptr(q), _ptr(k), _ptr(v), _ptr(out)),
                self.ctx._h)
 
 

@@ -342,6 +342,7 @@ void prepare_impl(psi_gqa* g, const uint32_t* req_slots, const uint32_t* token_i
                     "GQA request context does not fit the request page table");
         }
 
+        plan_weigh(g, req_slots, token_indices, cu_tokens, num_reqs);
         if (g->cfg.plan_mode == PSI_PLAN_REFERENCE) {
             g->plan = build_reference_plan(g->geo, *g->md, shape, variant.tiled_q != 0, token_indices, cu_tokens,
                                            num_reqs);
@@ -382,6 +383,8 @@ void prepare_impl(psi_gqa* g, const uint32_t* req_slots, const uint32_t* token_i
             cursor += pad_words(num_tokens);
             g->off_token_indices = cursor;
             cursor += pad_words(num_tokens);
+            g->off_weigh = cursor;
+            cursor += g->weigh.reqs.size() * kWeighRequestWords;
             place_plan(g->off, cursor, plan, chunk, device_items.size());
             if (g->has_merged) {
                 g->merged_off.scalars = cursor;
@@ -419,6 +422,9 @@ void prepare_impl(psi_gqa* g, const uint32_t* req_slots, const uint32_t* token_i
         std::copy(g->md->req_slots.begin(), g->md->req_slots.begin() + num_tokens, s + g->off_req_slots);
         std::copy(g->md->flat_token_indices.begin(), g->md->flat_token_indices.begin() + num_tokens,
                   s + g->off_token_indices);
+        s[kScalarWeighShort] = g->weigh.num_short;
+        s[kScalarWeighLong] = g->weigh.num_long;
+        std::memcpy(s + g->off_weigh, g->weigh.reqs.data(), g->weigh.reqs.size() * sizeof(WeighRequest));
         if (g->replay_reserved) {
             // launches run at the capacity grid: CTAs beyond the plan's find an empty range and a zero first item
             constexpr uint64_t kItemWords = sizeof(DeviceItem) / sizeof(uint32_t);

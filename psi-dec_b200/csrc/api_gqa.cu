@@ -71,6 +71,10 @@ int32_t psi_gqa_destroy(psi_gqa* g) {
         g->sync_words.release();
         g->xchg_local.release();
         g->norm_rope.release();
+        g->weigh.lse.release();
+        g->weigh.partials.release();
+        g->weigh.counters.release();
+        g->weigh.scores.release();
         for (cudaEvent_t e : g->pipe_events) (void)cudaEventDestroy(e);
         if (g->pipe_h2d != nullptr) (void)cudaStreamDestroy(g->pipe_h2d);
         if (g->pipe_d2h != nullptr) (void)cudaStreamDestroy(g->pipe_d2h);
@@ -100,6 +104,8 @@ static void reserved_layout(psi_gqa* g) {
     cursor += pad_words(t);
     g->off_token_indices = cursor;
     cursor += pad_words(t);
+    g->off_weigh = cursor;
+    cursor += (t + 2) * kWeighRequestWords;
     g->off.cta = cursor;
     cursor += pad_words(g->grid_cap + 2);
     g->off.first_items = cursor;

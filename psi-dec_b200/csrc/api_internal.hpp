@@ -19,6 +19,7 @@
 #include "kernels.cuh"
 #include "psi_cuda.h"
 #include "snapshot.hpp"
+#include "weigh_keys.hpp"
 
 namespace psi {
 
@@ -37,7 +38,7 @@ inline void cuda_check(cudaError_t err, const char* what) {
 constexpr uint32_t kWordAlign = 8;  // sections of the device metadata block start on 32-byte boundaries
 inline uint64_t pad_words(uint64_t n) { return (n + kWordAlign - 1) / kWordAlign * kWordAlign; }
 
-constexpr uint32_t kKernelClasses = 7;
+constexpr uint32_t kKernelClasses = 10;
 
 }  // namespace psi
 
@@ -83,7 +84,8 @@ struct LaunchScope {
         // last, so that nothing that can throw stands between the push and the destructor's pop
         static const char* const kNames[kKernelClasses] = {"psi kv_append",     "psi attend_map", "psi attend_reduce",
                                                            "psi combine",       "psi page_gather", "psi attend_chunk",
-                                                           "psi norm_rope_append"};
+                                                           "psi norm_rope_append", "psi weigh_keys", "psi evict",
+                                                           "psi linear_attend"};
         nvtxRangePushA(kernel_class < kKernelClasses ? kNames[kernel_class] : "psi launch");
     }
     ~LaunchScope() {
@@ -118,6 +120,11 @@ struct DeviceBuffer {
         if (ptr != nullptr) (void)cudaFree(ptr);
         ptr = nullptr;
         bytes = 0;
+    }
+    // The same once the stream's work on it is done.
+    void release_after(psi_ctx* ctx) {
+        if (ptr != nullptr) cuda_check(cudaStreamSynchronize(ctx->stream), "cudaStreamSynchronize");
+        release();
     }
 };
 
@@ -182,6 +189,21 @@ struct PlanOffsets {
 };
 }  // namespace psi
 
+// Key weights (psi_gqa_weigh_keys): the prepared batch as its kernels see it, and their scratch.
+struct psi_weigh_plan {
+    std::vector<psi::WeighRequest> reqs;
+    uint32_t num_short = 0, num_long = 0;
+    uint32_t short_rows = 0;             // most query rows of a KV head among the short runs
+    uint32_t max_keys = 0;
+    uint64_t tiles = 0, stats_items = 0, sum_items = 0, long_units = 0;
+    bool repeated = false;               // a slot appears twice in the batch
+    bool too_large = false;
+    bool captured = false;               // a captured launch sequence holds key-weight launches
+    std::vector<uint32_t> seen;          // by slot: the epoch that last named it
+    uint32_t epoch = 0;
+    psi::DeviceBuffer lse, partials, counters, scores;
+};
+
 struct psi_gqa {
     psi_ctx* ctx = nullptr;
     psi_gqa_config cfg{};
@@ -206,7 +228,7 @@ struct psi_gqa {
     uint64_t staging_words = 0;
     cudaEvent_t upload_done = nullptr;
     // section offsets (in words) of the block uploaded by the last prepare
-    uint64_t off_req_slots = 0, off_token_indices = 0;
+    uint64_t off_req_slots = 0, off_token_indices = 0, off_weigh = 0;
     psi::PlanOffsets off;
     // The plan with adjacent requests of one position merged (merge_one_position_runs), for launches that read this step's
     // K/V from their pages; beside the plan above, which fused launches take.  Under a replay reservation every launch
@@ -237,6 +259,7 @@ struct psi_gqa {
     psi_norm_rope_config norm_rope_cfg{};
     float norm_rope_attention_factor = 1.0f;
     bool has_norm_rope = false;
+    psi_weigh_plan weigh;
 };
 
 namespace psi {
@@ -303,6 +326,7 @@ constexpr uint64_t kHostPullTiles = 165;
 bool split_requests(const psi_gqa* g, const RequestRuns& runs, const ChunkRule& rule, std::vector<uint32_t>& decode_reqs,
                     std::vector<uint32_t>& chunk_reqs);
 ChunkRule chunk_rule(const psi_gqa* g, uint64_t handicap);
+void plan_weigh(psi_gqa* g, const uint32_t* req_slots, const uint32_t* token_indices, const uint32_t* cu_tokens, uint32_t num_reqs);
 void run_append(psi_gqa* g, psi_pages* pages, psi_table* table, uint32_t layer, const void* k, const void* v);
 // Device-side address of a pinned, device-mapped host buffer (16-byte aligned), or nullptr for any other memory.
 void* mapped_device_pointer(const void* host);

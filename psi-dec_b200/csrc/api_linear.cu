@@ -1,0 +1,194 @@
+// C ABI: linear attention with a decay for each head.
+#include "api_internal.hpp"
+#include "linear_attend.hpp"
+
+using namespace psi;
+
+struct psi_linear {
+    psi_ctx* ctx = nullptr;
+    psi_linear_config cfg{};
+    DeviceBuffer block;        // scalars | requests, at the same place from step to step
+    uint32_t* staging = nullptr;
+    cudaEvent_t upload_done = nullptr;
+    DeviceBuffer decays;       // [layers][Hv][kLinearDecays]
+    uint32_t num_steps = 0;    // requests of the prepared batch
+    bool prepared = false;
+    std::vector<uint32_t> reads, writes;  // by slot: readers of it in the batch at hand, and whether one writes it
+};
+
+namespace {
+
+uint64_t block_capacity(const psi_linear* l) { return kLinearScalarCount + uint64_t(l->cfg.max_tokens) * kLinearRequestWords; }
+
+}  // namespace
+
+extern "C" {
+
+int32_t psi_linear_create(psi_ctx* ctx, const psi_linear_config* config, psi_linear** out) {
+    if (ctx == nullptr) return PSI_ERR_INVALID_ARGUMENT;
+    return guarded(ctx, [&] {
+        require(out != nullptr && config != nullptr, "out and config must not be null");
+        *out = nullptr;
+        const psi_linear_config& c = *config;
+        require(c.num_k_heads > 0 && c.num_v_heads > 0, "linear attention head counts must be positive");
+        require(c.num_v_heads % c.num_k_heads == 0, "linear attention v heads must be a multiple of k heads");
+        require(c.key_dim > 0 && c.key_dim % 8 == 0 && c.key_dim <= kLinearMaxDim && c.value_dim > 0 && c.value_dim % 8 == 0 &&
+                    c.value_dim <= kLinearMaxDim,
+                "linear attention key_dim and value_dim must be multiples of 8 up to 256");
+        require(c.scale > 0.0f && std::isfinite(c.scale), "linear attention scale must be positive");
+        require(c.dtype <= PSI_DTYPE_F16, "unsupported linear attention dtype");
+        require(c.num_req_slots > 0 && c.num_layers > 0 && c.max_tokens > 0, "linear attention slots, layers and tokens must be positive");
+        require(uint64_t(c.max_tokens) * c.num_v_heads * 8 <= kU32Max, "linear attention batch exceeds the kernels' work counts");
+        require(!ctx->capturing, "a linear attention component cannot be created during stream capture");
+        ctx->bind();
+        auto l = std::make_unique<psi_linear>();
+        l->ctx = ctx;
+        l->cfg = c;
+        l->reads.assign(c.num_req_slots, 0);
+        l->writes.assign(c.num_req_slots, 0);
+        const uint64_t decays = uint64_t(c.num_layers) * c.num_v_heads;
+        std::vector<float> none(decays * kLinearDecays, 0.0f);  // lambda = 1
+        for (uint64_t i = 0; i < decays; ++i) none[i * kLinearDecays] = 1.0f;
+        try {
+            l->block.ensure(ctx, block_capacity(l.get()) * sizeof(uint32_t), true);
+            l->decays.ensure(ctx, none.size() * sizeof(float), false);
+            cuda_check(cudaMemcpyAsync(l->decays.ptr, none.data(), none.size() * sizeof(float), cudaMemcpyHostToDevice, ctx->stream),
+                       "cudaMemcpyAsync");  // pageable source: staged before the call returns
+            cuda_check(cudaMallocHost(reinterpret_cast<void**>(&l->staging), block_capacity(l.get()) * sizeof(uint32_t)), "cudaMallocHost");
+            cuda_check(cudaEventCreateWithFlags(&l->upload_done, cudaEventDisableTiming), "cudaEventCreateWithFlags");
+        } catch (...) {
+            l->block.release();
+            l->decays.release();
+            if (l->staging != nullptr) (void)cudaFreeHost(l->staging);
+            throw;
+        }
+        *out = l.release();
+    });
+}
+
+int32_t psi_linear_destroy(psi_linear* l) {
+    if (l == nullptr) return PSI_OK;
+    const int32_t status = guarded(l->ctx, [&] {
+        l->ctx->bind();
+        (void)cudaStreamSynchronize(l->ctx->stream);
+        l->block.release();
+        l->decays.release();
+        if (l->staging != nullptr) (void)cudaFreeHost(l->staging);
+        if (l->upload_done != nullptr) (void)cudaEventDestroy(l->upload_done);
+    });
+    delete l;
+    return status;
+}
+
+int32_t psi_linear_set_decay(psi_linear* l, uint32_t layer, const float* log_decay) {
+    if (l == nullptr) return PSI_ERR_INVALID_ARGUMENT;
+    return guarded(l->ctx, [&] {
+        psi_ctx* ctx = l->ctx;
+        require(log_decay != nullptr, "log_decay must not be null");
+        require(layer < l->cfg.num_layers, "linear attention layer out of range");
+        require(!ctx->capturing, "psi_linear_set_decay uploads the decays and stays outside captured graphs");
+        const uint32_t heads = l->cfg.num_v_heads;
+        std::vector<float> parts(uint64_t(heads) * kLinearDecays);
+        for (uint32_t h = 0; h < heads; ++h) {
+            require(std::isfinite(log_decay[h]) && log_decay[h] <= 0.0f, "log_decay must be finite and not positive");
+            const double lambda = std::exp(double(log_decay[h]));
+            parts[h * kLinearDecays] = float(lambda);
+            parts[h * kLinearDecays + 1] = float(lambda - double(float(lambda)));
+            parts[h * kLinearDecays + 2] = log_decay[h];
+        }
+        ctx->bind();
+        cuda_check(cudaMemcpyAsync(static_cast<float*>(l->decays.ptr) + uint64_t(layer) * heads * kLinearDecays, parts.data(),
+                                   parts.size() * sizeof(float), cudaMemcpyHostToDevice, ctx->stream),
+                   "cudaMemcpyAsync");  // pageable source: staged before the call returns
+    });
+}
+
+int32_t psi_linear_prepare(psi_linear* l, const uint32_t* req_slots, const uint32_t* out_slots, const uint32_t* token_indices,
+                           const uint32_t* cu_tokens, uint32_t num_reqs) {
+    if (l == nullptr) return PSI_ERR_INVALID_ARGUMENT;
+    return guarded(l->ctx, [&] {
+        psi_ctx* ctx = l->ctx;
+        require(!ctx->capturing, "psi_linear_prepare uploads the step's batch and stays outside captured graphs");
+        require(req_slots != nullptr && token_indices != nullptr && cu_tokens != nullptr, "metadata inputs must not be null");
+        require(num_reqs > 0, "linear attention batch requires tokens");
+        require(cu_tokens[0] == 0, "linear attention batch cu_tokens must start at zero");
+        for (uint32_t r = 0; r < num_reqs; ++r)
+            require(cu_tokens[r] <= cu_tokens[r + 1], "linear attention batch cu_tokens must be nondecreasing");
+        require(cu_tokens[num_reqs] > 0, "linear attention batch requires tokens");
+        require(cu_tokens[num_reqs] <= l->cfg.max_tokens, "linear attention batch exceeds the token capacity");
+        const uint32_t* outs = out_slots != nullptr ? out_slots : req_slots;
+        for (uint32_t r = 0; r < num_reqs; ++r)
+            require(req_slots[r] < l->cfg.num_req_slots && outs[r] < l->cfg.num_req_slots, "linear attention req_slot out of range");
+        l->prepared = false;
+        // a slot is written by one request at most, and then read by none other
+        std::fill(l->reads.begin(), l->reads.end(), 0u);
+        std::fill(l->writes.begin(), l->writes.end(), 0u);
+        for (uint32_t r = 0; r < num_reqs; ++r) {
+            if (cu_tokens[r] == cu_tokens[r + 1]) continue;
+            require(l->writes[outs[r]] == 0, "two requests would write the state of one slot");
+            l->writes[outs[r]] = 1;
+            if (token_indices[r] > 0) l->reads[req_slots[r]] += 1;
+        }
+        for (uint32_t r = 0; r < num_reqs; ++r) {
+            if (cu_tokens[r] == cu_tokens[r + 1]) continue;
+            const uint32_t own = outs[r] == req_slots[r] && token_indices[r] > 0 ? 1 : 0;
+            require(l->reads[outs[r]] == own, "a request would write the state that another one reads");
+        }
+        ctx->bind();
+        cuda_check(cudaEventSynchronize(l->upload_done), "cudaEventSynchronize");  // previous upload left staging
+        std::fill(l->staging, l->staging + kLinearScalarCount, 0u);
+        auto* reqs = reinterpret_cast<LinearRequest*>(l->staging + kLinearScalarCount);
+        uint32_t n = 0;
+        for (uint32_t r = 0; r < num_reqs; ++r) {
+            const uint32_t q_len = cu_tokens[r + 1] - cu_tokens[r];
+            if (q_len > 0) reqs[n++] = LinearRequest{req_slots[r], outs[r], token_indices[r] == 0 ? 1u : 0u, q_len, cu_tokens[r], {0, 0, 0}};
+        }
+        l->staging[kLinearNumSteps] = n;
+        cuda_check(cudaMemcpyAsync(l->block.ptr, l->staging, (kLinearScalarCount + n * kLinearRequestWords) * sizeof(uint32_t),
+                                   cudaMemcpyHostToDevice, ctx->stream),
+                   "cudaMemcpyAsync");
+        cuda_check(cudaEventRecord(l->upload_done, ctx->stream), "cudaEventRecord");
+        l->num_steps = n;
+        l->prepared = true;
+    });
+}
+
+int32_t psi_linear_attend(psi_linear* l, uint32_t layer, float* states, const void* q, const void* k, const void* v, void* out) {
+    if (l == nullptr) return PSI_ERR_INVALID_ARGUMENT;
+    return guarded(l->ctx, [&] {
+        psi_ctx* ctx = l->ctx;
+        require(l->prepared, "a linear attention batch must be prepared before recording");
+        require(states != nullptr && q != nullptr && k != nullptr && v != nullptr && out != nullptr, "linear attention buffers must not be null");
+        require(layer < l->cfg.num_layers, "linear attention layer out of range");
+        require((reinterpret_cast<uintptr_t>(states) & 15u) == 0, "linear attention states must be 16-byte aligned");
+        const uint32_t esz = dtype_bytes(l->cfg.dtype);
+        require((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out)) % esz == 0,
+                "linear attention buffers must be aligned to their elements");
+        ctx->bind();
+        LinearParams p{};
+        p.scalars = static_cast<const uint32_t*>(l->block.ptr);
+        p.reqs = reinterpret_cast<const LinearRequest*>(p.scalars + kLinearScalarCount);
+        p.decays = static_cast<const float*>(l->decays.ptr) + uint64_t(layer) * l->cfg.num_v_heads * kLinearDecays;
+        p.states = states;
+        p.q = q;
+        p.k = k;
+        p.v = v;
+        p.out = out;
+        p.layer = layer;
+        p.num_layers = l->cfg.num_layers;
+        p.num_k_heads = l->cfg.num_k_heads;
+        p.num_v_heads = l->cfg.num_v_heads;
+        p.key_dim = l->cfg.key_dim;
+        p.value_dim = l->cfg.value_dim;
+        p.dtype = l->cfg.dtype;
+        p.scale = l->cfg.scale;
+        const uint64_t wave = static_cast<uint64_t>(ctx->sm_count) * 16;
+        const uint64_t per_request = uint64_t(l->cfg.num_v_heads) * linear_step_slices(l->cfg.value_dim);
+        // a captured launch has to be right for every later batch: its grid does not depend on this one
+        const uint64_t items = (ctx->capturing ? uint64_t(l->cfg.max_tokens) : l->num_steps) * per_request;
+        LaunchScope scope(ctx, PSI_KERNEL_CLASS_LINEAR);
+        cuda_check(launch_linear_step(p, static_cast<uint32_t>(std::min(items, wave)), ctx->stream), "linear attention launch");
+    });
+}
+
+}  // extern "C"

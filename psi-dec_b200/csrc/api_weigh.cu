@@ -1,0 +1,254 @@
+// C ABI: attention weight gathered by cached keys, and eviction from the cache by it.
+#include "api_internal.hpp"
+#include "evict.hpp"
+#include "weigh_keys.hpp"
+
+using namespace psi;
+
+namespace psi {
+
+// The batch as the key-weight kernels see it (WeighRequest): short runs, their end, long runs, their end.  A batch whose
+// counts leave 32 bits is marked, and refused by psi_gqa_weigh_keys alone.
+void plan_weigh(psi_gqa* g, const uint32_t* req_slots, const uint32_t* token_indices, const uint32_t* cu_tokens, uint32_t num_reqs) {
+    psi_weigh_plan& w = g->weigh;
+    w.reqs.clear();
+    w.num_short = w.num_long = w.max_keys = w.short_rows = 0;
+    w.long_units = 0;
+    w.repeated = w.too_large = false;
+    const uint32_t group = g->cfg.num_q_heads / g->cfg.num_kv_heads, heads = g->cfg.num_kv_heads;
+    const bool tensor = weigh_on_tensor_cores(g->cfg.dtype, g->cfg.head_dim);
+    const uint32_t block = tensor ? kWeighBlock : kWeighAnyRows;
+    if (w.seen.empty()) w.seen.assign(g->cfg.layout.num_req_slots, 0);
+    w.epoch += 1;
+    if (w.epoch == 0) {
+        std::fill(w.seen.begin(), w.seen.end(), 0u);
+        w.epoch = 1;
+    }
+    uint64_t cu0 = 0, cu1 = 0;
+    for (int pass = 0; pass < 2; ++pass) {  // 0: short runs, 1: long ones
+        cu0 = cu1 = 0;
+        for (uint32_t r = 0; r < num_reqs; ++r) {
+            const uint32_t q_len = cu_tokens[r + 1] - cu_tokens[r];
+            if (q_len == 0) continue;
+            const uint64_t rows = uint64_t(q_len) * group;
+            const bool is_short = tensor && rows <= kWeighShortRows;
+            if (is_short != (pass == 0)) continue;
+            if (w.seen[req_slots[r]] == w.epoch) w.repeated = true;
+            w.seen[req_slots[r]] = w.epoch;
+            const uint32_t keys = token_indices[r] + q_len;
+            WeighRequest rq{req_slots[r], token_indices[r], q_len, cu_tokens[r], keys, uint32_t(cu0), uint32_t(cu1), uint32_t(w.long_units)};
+            w.reqs.push_back(rq);
+            w.max_keys = std::max(w.max_keys, keys);
+            if (is_short) {
+                w.num_short += 1;
+                w.short_rows = std::max(w.short_rows, uint32_t(rows));
+                cu0 += (uint64_t(keys) + kWeighTile - 1) / kWeighTile * heads;
+            } else {
+                w.num_long += 1;
+                const uint64_t units = (rows + block - 1) / block * heads;
+                w.long_units += units;
+                cu0 += units * weigh_pieces(keys);
+                cu1 += (uint64_t(keys) + kWeighBlock - 1) / kWeighBlock * heads;
+            }
+        }
+        WeighRequest end{};
+        end.cu0 = uint32_t(cu0);
+        end.cu1 = uint32_t(cu1);
+        w.reqs.push_back(end);
+        w.too_large = w.too_large || cu0 > kU32Max || cu1 > kU32Max || w.long_units > kU32Max;
+        if (pass == 0) w.tiles = cu0;
+    }
+    w.stats_items = cu0;
+    w.sum_items = cu1;
+    require(!w.captured || (!w.repeated && !w.too_large),
+            "a request slot appears twice in the batch: the captured key-weight launches cannot add to its keys twice at once");
+}
+
+}  // namespace psi
+
+namespace {
+
+uint64_t table_tokens(const psi_gqa* g) {
+    return uint64_t(g->cfg.layout.num_blocks) * g->cfg.layout.num_page_ids_per_block * g->tokens_per_page;
+}
+
+void run_pass(psi_gqa* g, const WeighParams& p, WeighPass pass, uint64_t ctas) {
+    LaunchScope scope(g->ctx, PSI_KERNEL_CLASS_WEIGH);
+    cuda_check(launch_weigh(p, pass, static_cast<uint32_t>(ctas), g->ctx->stream), "key weight launch");
+}
+
+// The largest unit of a row copy: what the rows' bytes and the arena's address are multiples of.
+uint32_t copy_unit(const PageGeometry& geo) {
+    const uint64_t at = reinterpret_cast<uintptr_t>(geo.pages) | (uint64_t(geo.head_dim) * geo.elem_bytes);
+    return at % 16 == 0 ? 16u : at % 4 == 0 ? 4u : 2u;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint32_t layer, const void* q, float* weights,
+                           uint64_t weights_stride) {
+    if (g == nullptr) return PSI_ERR_INVALID_ARGUMENT;
+    return guarded(g->ctx, [&] {
+        psi_ctx* ctx = g->ctx;
+        psi_weigh_plan& w = g->weigh;
+        require(g->prepared, "GQA batch metadata must be updated before recording");
+        require(q != nullptr && weights != nullptr, "q and weights must not be null");
+        require(!w.repeated, "a request slot appears twice in the batch: its keys cannot gather weight from two requests at once");
+        require(!w.too_large, "the batch exceeds the key-weight kernels' work counts");
+        WeighParams p{};
+        p.geo = page_geometry(g, pages, table, layer);
+        const bool tensor = weigh_on_tensor_cores(g->cfg.dtype, g->cfg.head_dim);
+        require(!tensor || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(p.geo.pages)) & 15u) == 0,
+                "q and the page arena must be 16-byte aligned");
+        require((reinterpret_cast<uintptr_t>(weights) & 3u) == 0, "weights must be 4-byte aligned");
+        require(reinterpret_cast<uintptr_t>(q) % dtype_bytes(g->cfg.dtype) == 0, "q must be aligned to its elements");
+        require(weights_stride >= w.max_keys, "the weights' row stride must hold every key of the batch");
+        const bool fixed = g->replay_reserved;
+        require(!ctx->capturing || fixed, "reserve replay capacity before capturing key-weight launches");
+        require(!ctx->capturing || weights_stride >= table_tokens(g),
+                "captured key-weight launches need rows of weights as long as the page table's");
+        ctx->bind();
+        const uint32_t heads = g->cfg.num_kv_heads, group = g->cfg.num_q_heads / heads;
+        const uint64_t sms = static_cast<uint64_t>(ctx->sm_count);
+        const uint32_t block = tensor ? kWeighBlock : kWeighAnyRows;
+        const bool can_short = tensor, can_long = !tensor || uint64_t(g->cfg.max_tokens) * group > kWeighShortRows;
+        // one wave of the short-run kernel's workers
+        const uint64_t short_wave = sms * (g->cfg.head_dim <= 128 ? 2 : 1);
+        const uint64_t short_ctas = fixed ? (can_short ? short_wave : 0) : std::min<uint64_t>(short_wave, (w.tiles + 7) / 8);
+        uint64_t short_units = uint64_t(w.num_short) * heads, long_units = w.long_units, stats_items = w.stats_items;
+        if (fixed) {
+            short_units = can_short ? uint64_t(g->cfg.max_tokens) * heads : 0;
+            const uint64_t rows = uint64_t(g->cfg.max_tokens) * group;
+            long_units = can_long ? (rows / block + (tensor ? rows / (kWeighShortRows + 1) : g->cfg.max_tokens) + 1) * heads : 0;
+            stats_items = long_units * weigh_pieces(static_cast<uint32_t>(std::min<uint64_t>(table_tokens(g), kU32Max)));
+        }
+        const uint64_t short_slots = (short_ctas * 8 + short_units) * 16, long_slots = stats_items * block;
+        const uint64_t partial_bytes = (short_slots + long_slots) * sizeof(float2);
+        const uint64_t counter_words = short_units + long_units;
+        if (ctx->capturing) {
+            require(w.lse.ptr != nullptr && partial_bytes <= w.partials.bytes && counter_words * sizeof(uint32_t) <= w.counters.bytes,
+                    "call psi_gqa_weigh_keys once after the replay reservation and before the capture: it allocates its scratch then");
+        } else {
+            require(!fixed || partial_bytes <= (2ull << 30),
+                    "the replay reservation needs more than 2 GiB of key-weight scratch for this max_tokens: create the component with "
+                    "the largest batch the replayed steps carry");
+            w.lse.ensure(ctx, uint64_t(g->cfg.max_tokens) * g->cfg.num_q_heads * sizeof(float), false);
+            w.partials.ensure(ctx, partial_bytes > w.partials.bytes ? std::max<uint64_t>(partial_bytes * 3 / 2, 1 << 16) : partial_bytes, false);
+            if (counter_words * sizeof(uint32_t) > w.counters.bytes) {
+                w.counters.release_after(ctx);  // counters restart from zero at their new size
+                w.counters.ensure(ctx, std::max<uint64_t>(counter_words * 6, 1 << 12), true);
+            }
+        }
+        p.q = q;
+        p.weights = weights;
+        p.stride = weights_stride;
+        p.reqs = reinterpret_cast<const WeighRequest*>(block_words(g, g->off_weigh));
+        p.scalars = block_words(g, 0);
+        p.lse = static_cast<float*>(w.lse.ptr);
+        p.partials = static_cast<float2*>(w.partials.ptr);
+        p.long_partials_at = short_slots;
+        p.counters = static_cast<uint32_t*>(w.counters.ptr);
+        p.long_counters_at = short_units;
+        p.group = group;
+        p.num_q_heads = g->cfg.num_q_heads;
+        p.dtype = g->cfg.dtype;
+        p.scale_log2 = g->cfg.scale * 1.4426950408889634f;
+        p.score_rows = w.short_rows <= 8 ? 8 : 16;
+        bool keep_scores = false;
+        if (short_ctas > 0 && !fixed) {
+            // The scores of short runs stay in scratch between the passes; beyond 2 GiB, or where the device has no room left,
+            // the second pass reads the keys again instead.
+            const uint64_t bytes = w.tiles * kWeighTile * p.score_rows * sizeof(float);
+            keep_scores = bytes <= (2ull << 30);
+            if (keep_scores && bytes > w.scores.bytes) {
+                try {
+                    w.scores.ensure(ctx, bytes + bytes / 2, false);
+                } catch (const ExhaustedError&) {
+                    keep_scores = false;
+                }
+            }
+            p.scores = static_cast<float*>(w.scores.ptr);
+        }
+        if (ctx->capturing) w.captured = true;
+        if (short_ctas > 0) run_pass(g, p, keep_scores ? WeighPass::kShortStatsScores : WeighPass::kShortStats, short_ctas);
+        const uint64_t stats_ctas = fixed ? (can_long ? sms * 8 : 0) : std::min<uint64_t>(sms * 8, w.stats_items);
+        const uint64_t sum_ctas = fixed ? stats_ctas : std::min<uint64_t>(sms * 8, w.sum_items);
+        if (stats_ctas > 0) run_pass(g, p, WeighPass::kLongStats, stats_ctas);
+        if (short_ctas > 0) {
+            const uint64_t ctas = keep_scores ? std::min<uint64_t>(sms * 8, (w.tiles + 7) / 8) : short_ctas;
+            run_pass(g, p, keep_scores ? WeighPass::kShortSumScores : WeighPass::kShortSumAgain, ctas);
+        }
+        if (stats_ctas > 0) run_pass(g, p, WeighPass::kLongSum, sum_ctas);
+    });
+}
+
+int32_t psi_gqa_evict(psi_gqa* g, psi_pages* pages, psi_table* table, uint32_t layer, const uint32_t* src_slots,
+                      const uint32_t* dst_slots, const uint32_t* lengths, const uint32_t* keeps, uint32_t num_reqs, uint32_t recent,
+                      const float* weights, float* weights_out, uint64_t weights_stride, uint32_t* kept, uint64_t kept_stride) {
+    if (g == nullptr) return PSI_ERR_INVALID_ARGUMENT;
+    return guarded(g->ctx, [&] {
+        psi_ctx* ctx = g->ctx;
+        require(!ctx->capturing, "psi_gqa_evict takes its sizes from host arrays and stays outside captured graphs");
+        require(num_reqs == 0 || (src_slots != nullptr && dst_slots != nullptr && lengths != nullptr && keeps != nullptr),
+                "eviction inputs must not be null");
+        require(weights != nullptr && weights_out != nullptr && kept != nullptr, "weights, weights_out and kept must not be null");
+        require(((reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(weights_out) | reinterpret_cast<uintptr_t>(kept)) & 3u) == 0,
+                "weights and kept must be 4-byte aligned");
+        require(g->cfg.num_kv_heads <= 32767, "eviction launches take up to 32767 KV heads");
+        EvictParams p{};
+        p.geo = page_geometry(g, pages, table, layer);
+        require(reinterpret_cast<uintptr_t>(p.geo.pages) % p.geo.elem_bytes == 0, "the page arena must be aligned to its elements");
+        const uint64_t capacity = table_tokens(g);
+        const uint32_t slots = g->cfg.layout.num_req_slots;
+        std::vector<uint32_t> role(slots, 0);  // 1 + r: slot is the source of request r
+        std::vector<bool> taken(slots, false);
+        for (uint32_t r = 0; r < num_reqs; ++r) {
+            require(src_slots[r] < slots && dst_slots[r] < slots, "GQA request page table req_slot out of range");
+            require(lengths[r] <= capacity, "eviction length does not fit the request page table");
+            require(lengths[r] <= weights_stride, "the weights' row stride must hold every key of the batch");
+            require(keeps[r] <= lengths[r], "eviction cannot keep more keys than the request has");
+            require(keeps[r] <= kept_stride, "the kept rows' stride must hold every kept key");
+            require(role[src_slots[r]] == 0, "a request slot is evicted from twice in one call");
+            role[src_slots[r]] = 1 + r;
+        }
+        for (uint32_t r = 0; r < num_reqs; ++r) {
+            require(!taken[dst_slots[r]], "two requests would move to one slot");
+            taken[dst_slots[r]] = true;
+            require(role[dst_slots[r]] == 0 || role[dst_slots[r]] == 1 + r, "a request would move to a slot that another one is read from");
+        }
+        ctx->bind();
+        p.weights = weights;
+        p.weights_out = weights_out;
+        p.stride = weights_stride;
+        p.kept_stride = kept_stride;
+        p.recent = recent;
+        p.unit_bytes = copy_unit(p.geo);
+        const uint32_t wave = static_cast<uint32_t>(ctx->sm_count) * 4;
+        for (uint32_t first = 0; first < num_reqs; first += kEvictBatch) {
+            p.num_reqs = std::min(kEvictBatch, num_reqs - first);
+            p.kept = kept + uint64_t(first) * g->cfg.num_kv_heads * kept_stride;
+            bool in_place = false, apart = false;
+            for (uint32_t r = 0; r < p.num_reqs; ++r) {
+                const uint32_t at = first + r;
+                p.reqs[r] = EvictRequest{src_slots[at], dst_slots[at], lengths[at], keeps[at]};
+                const bool same = src_slots[at] == dst_slots[at];
+                in_place = in_place || (same && keeps[at] > 0 && keeps[at] < lengths[at]);
+                apart = apart || (!same && keeps[at] > 0);
+            }
+            {
+                LaunchScope scope(ctx, PSI_KERNEL_CLASS_EVICT);
+                cuda_check(launch_evict_select(p, ctx->stream), "eviction selection launch");
+            }
+            for (uint32_t way = 0; way < 2; ++way) {
+                if (!(way == 0 ? apart : in_place)) continue;
+                p.in_place = way;
+                LaunchScope scope(ctx, PSI_KERNEL_CLASS_EVICT);
+                cuda_check(launch_evict_move(p, wave, ctx->stream), "eviction move launch");
+            }
+        }
+    });
+}
+
+}  // extern "C"

@@ -16,6 +16,8 @@ enum ScalarSlot : uint32_t {
     kScalarNumReduces = 2,
     kScalarNumChunkCtas = 3,
     kScalarFineChunks = 4,        // the chunk plan's items want their weights in two parts (tcgen05 kernel)
+    kScalarWeighShort = 5,        // key weights: requests on the short-run kernel, and on the long-run kernels
+    kScalarWeighLong = 6,
     kScalarCount = 8
 };
 

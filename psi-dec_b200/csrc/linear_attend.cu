@@ -1,0 +1,119 @@
+// Linear attention with a decay for each head (psi_linear_attend): per value head, with lambda = exp(log_decay),
+//
+//   S_t = lambda S_{t-1} + k_t^T v_t        o_t = scale q_t S_t        S: f32 [Dk][Dv]
+//
+// linear_step_kernel, the recurrent form: a CTA takes 32 columns of one head's state of one request into registers, goes through
+// the request's tokens and writes the columns back: bound by the state's bytes, read and written once for the whole run.  A
+// decay close to one that is rounded to f32 would be off by 2^-25 a token, and all in the same direction; it is held as two f32
+// parts instead (lambda = hi + lo to 48 bits), one more multiply-add for each element and token.
+#include "device_common.cuh"
+#include "launch_util.hpp"
+#include "linear_attend.hpp"
+
+namespace psi {
+
+namespace {
+
+constexpr uint32_t kStepThreads = 128;
+constexpr uint32_t kStepColumns = 32;                       // of the state in one CTA: eight threads of four
+constexpr uint32_t kStepRowGroups = kStepThreads / 8;       // thread (group, four columns) holds rows group + 16 j
+constexpr uint32_t kStepTokens = 8;                         // tokens whose rows are in shared memory at once
+
+__device__ __forceinline__ float* state_of(const LinearParams& p, uint32_t slot, uint32_t head) {
+    return p.states + ((uint64_t(slot) * p.num_layers + p.layer) * p.num_v_heads + head) * p.key_dim * p.value_dim;
+}
+
+template <int kRows>  // of the state in one thread: key_dim <= 16 kRows
+__global__ __launch_bounds__(kStepThreads) void linear_step_kernel(const LinearParams p) {
+    __shared__ float q_rows[kStepTokens][kRows * 16], k_rows[kStepTokens][kRows * 16];
+    __shared__ __align__(16) float v_cols[kStepTokens][kStepColumns];
+    __shared__ __align__(16) float sums[kStepTokens][kStepThreads / 32][kStepColumns];
+    await_previous_kernel();
+    const uint32_t slices = (p.value_dim + kStepColumns - 1) / kStepColumns;
+    const uint32_t total = p.scalars[kLinearNumSteps] * p.num_v_heads * slices;
+    const uint32_t share = p.num_v_heads / p.num_k_heads;
+    const uint32_t group = threadIdx.x >> 3, quad = threadIdx.x & 7u, warp = threadIdx.x >> 5;
+    for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
+        const uint32_t slice = item % slices, head = item / slices % p.num_v_heads;
+        const LinearRequest rq = p.reqs[item / slices / p.num_v_heads];
+        const uint32_t col = slice * kStepColumns + 4u * quad;
+        const bool live = col < p.value_dim;  // value_dim is a multiple of eight
+        const float* from = state_of(p, rq.src, head);
+        float4 s[kRows];
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) {
+            const uint32_t row = group + kStepRowGroups * j;
+            s[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (rq.fresh == 0 && live && row < p.key_dim) s[j] = *reinterpret_cast<const float4*>(from + uint64_t(row) * p.value_dim + col);
+        }
+        const float hi = p.decays[head * kLinearDecays], lo = p.decays[head * kLinearDecays + 1];
+        for (uint32_t t0 = 0; t0 < rq.q_len; t0 += kStepTokens) {
+            const uint32_t tokens = min(kStepTokens, rq.q_len - t0);
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < tokens * kRows * 16u; i += kStepThreads) {
+                const uint32_t t = i / (kRows * 16u), d = i % (kRows * 16u);
+                const uint64_t at = (uint64_t(rq.flat_begin + t0 + t) * p.num_k_heads + head / share) * p.key_dim + d;
+                q_rows[t][d] = d < p.key_dim ? load_as_float(p.q, at, p.dtype) : 0.0f;
+                k_rows[t][d] = d < p.key_dim ? load_as_float(p.k, at, p.dtype) : 0.0f;
+            }
+            for (uint32_t i = threadIdx.x; i < tokens * kStepColumns; i += kStepThreads) {
+                const uint32_t t = i / kStepColumns, c = slice * kStepColumns + i % kStepColumns;
+                v_cols[t][i % kStepColumns] =
+                    c < p.value_dim ? load_as_float(p.v, (uint64_t(rq.flat_begin + t0 + t) * p.num_v_heads + head) * p.value_dim + c, p.dtype) : 0.0f;
+            }
+            __syncthreads();
+            for (uint32_t t = 0; t < tokens; ++t) {
+                const float4 v = *reinterpret_cast<const float4*>(&v_cols[t][4u * quad]);
+                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int j = 0; j < kRows; ++j) {
+                    const float k = k_rows[t][group + kStepRowGroups * j], q = q_rows[t][group + kStepRowGroups * j];
+                    s[j].x = fmaf(hi, s[j].x, fmaf(lo, s[j].x, k * v.x));
+                    s[j].y = fmaf(hi, s[j].y, fmaf(lo, s[j].y, k * v.y));
+                    s[j].z = fmaf(hi, s[j].z, fmaf(lo, s[j].z, k * v.z));
+                    s[j].w = fmaf(hi, s[j].w, fmaf(lo, s[j].w, k * v.w));
+                    o.x = fmaf(q, s[j].x, o.x);
+                    o.y = fmaf(q, s[j].y, o.y);
+                    o.z = fmaf(q, s[j].z, o.z);
+                    o.w = fmaf(q, s[j].w, o.w);
+                }
+#pragma unroll
+                for (int x = 8; x < 32; x <<= 1) {
+                    o.x += __shfl_xor_sync(0xFFFFFFFFu, o.x, x);
+                    o.y += __shfl_xor_sync(0xFFFFFFFFu, o.y, x);
+                    o.z += __shfl_xor_sync(0xFFFFFFFFu, o.z, x);
+                    o.w += __shfl_xor_sync(0xFFFFFFFFu, o.w, x);
+                }
+                if ((threadIdx.x & 31u) < 8u) *reinterpret_cast<float4*>(&sums[t][warp][4u * quad]) = o;
+            }
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < tokens * kStepColumns; i += kStepThreads) {
+                const uint32_t t = i / kStepColumns, c = i % kStepColumns;
+                float o = 0.0f;
+#pragma unroll
+                for (uint32_t x = 0; x < kStepThreads / 32; ++x) o += sums[t][x][c];
+                if (slice * kStepColumns + c < p.value_dim)
+                    store_from_float(p.out, (uint64_t(rq.flat_begin + t0 + t) * p.num_v_heads + head) * p.value_dim + slice * kStepColumns + c,
+                                     p.dtype, o * p.scale);
+            }
+        }
+        float* to = state_of(p, rq.dst, head);
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) {
+            const uint32_t row = group + kStepRowGroups * j;
+            if (live && row < p.key_dim) *reinterpret_cast<float4*>(to + uint64_t(row) * p.value_dim + col) = s[j];
+        }
+    }
+}
+
+}  // namespace
+
+uint32_t linear_step_slices(uint32_t value_dim) { return (value_dim + kStepColumns - 1) / kStepColumns; }
+
+cudaError_t launch_linear_step(const LinearParams& p, uint32_t ctas, cudaStream_t stream) {
+    if (p.key_dim <= 64) return launch_overlapped(linear_step_kernel<4>, dim3(ctas), dim3(kStepThreads), 0, stream, p);
+    if (p.key_dim <= 128) return launch_overlapped(linear_step_kernel<8>, dim3(ctas), dim3(kStepThreads), 0, stream, p);
+    return launch_overlapped(linear_step_kernel<16>, dim3(ctas), dim3(kStepThreads), 0, stream, p);
+}
+
+}  // namespace psi

@@ -1,0 +1,755 @@
+// Attention weight gathered by each cached key (psi_gqa_weigh_keys).
+//
+//   weights[slot][kv head][j] += sum over the request's query rows r (token i of the run, head of the group) of
+//                                exp(scale q_r . k_j - M_r) / L_r        for j <= token_index + i
+//
+// with M_r and L_r the maximum and the exponential sum of row r's scores.  A row without a finite maximum or sum adds nothing.
+// Two passes, since no weight is known before its row's sum is: the first finds log2-domain normalisers, the second adds up
+// columns.  Both keep f32 scores; every key's sum is worked out by one thread group in one order, so results repeat bit for bit.
+//
+//   weigh_short_kernel   runs of up to 16 rows (decode, drafts): bound by the K bytes.  One warp is one worker with an equal
+//                        share of the batch's 32-key tiles.  Products do not depend on the order of the columns of q and k, so
+//                        a lane takes 16 consecutive bytes of a key row as the operands of two m16n8k16 steps, and the
+//                        same bytes of the query rows: K goes from HBM to registers with no shared memory and no barrier, for any
+//                        page size.  The first pass leaves its scores in scratch, 4 bytes a row and key against 2 head_dim
+//                        bytes a key, so that K is read once; where there is no scratch (captured launches, very
+//                        large batches) the second pass reads K again.
+//   weigh_stats_kernel,  longer runs: 64 rows (first pass) or 64 keys (second pass) stay in registers as the A operand, blocks
+//   weigh_sum_kernel     of 64 keys or rows pass through shared memory as the B operand.  In the second pass the keys are the
+//                        rows of the product, so a column sum stays inside a thread until its end.
+//   weigh_*_any_kernel   f32 and head dims that are no multiple of eight: the same two passes in f32 on the CUDA cores.
+#include "mma_common.cuh"
+#include "launch_util.hpp"
+#include "weigh_keys.hpp"
+
+namespace psi {
+
+namespace {
+
+constexpr float kInf = INFINITY;
+
+__device__ __forceinline__ uint4 ld_stream(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// The request whose work holds `index`: the last one whose prefix (`which` 0: cu0, 1: cu1) is at or below it.
+template <int kWhich>
+__device__ __forceinline__ uint32_t find_request(const WeighRequest* reqs, uint32_t count, uint32_t index) {
+    uint32_t lo = 0, hi = count;  // invariant: prefix[lo] <= index < prefix[hi]
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if ((kWhich == 0 ? reqs[mid].cu0 : reqs[mid].cu1) <= index) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// (maximum, sum) of a row's scores in the log2 domain; an empty one is (-inf, 0).
+struct Stat {
+    float m, l;
+    __device__ __forceinline__ void join(float m2, float l2) {
+        const float top = fmaxf(m, m2);
+        const float base = top == -kInf ? 0.0f : top;
+        l = l * exp2f(m - base) + l2 * exp2f(m2 - base);
+        m = top;
+    }
+    // The normaliser subtracted from the row's scores: +inf tells that the row adds nothing.
+    __device__ __forceinline__ float lse() const {
+        const float v = m + log2f(l);
+        return l > 0.0f && fabsf(v) < kInf ? v : kInf;
+    }
+};
+
+__device__ __forceinline__ float weight_of(float score, float lse) { return lse < kInf ? exp2f(score - lse) : 0.0f; }
+
+// Query row r of a request and KV head as (flat token, head) row of q.
+__device__ __forceinline__ uint64_t query_row(const WeighParams& p, const WeighRequest& rq, uint32_t head, uint32_t r) {
+    return uint64_t(rq.flat_begin + r / p.group) * p.num_q_heads + head * p.group + r % p.group;
+}
+
+// Keys that row r sees.
+__device__ __forceinline__ uint32_t row_limit(const WeighParams& p, const WeighRequest& rq, uint32_t r) {
+    return rq.first_pos + r / p.group + 1;
+}
+
+// 16-byte chunks of a 16-bit row that a lane holds: chunk (lane & 3) + 4 i for i < NC, zeros beyond the row.
+template <int NC>
+__device__ __forceinline__ void load_row(uint4 (&x)[NC], const uint4* row, uint32_t lane_chunk, uint32_t chunks) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const uint32_t c = lane_chunk + 4u * i;
+        x[i] = c < chunks ? ld_stream(row + c) : make_uint4(0, 0, 0, 0);
+    }
+}
+
+// A operand: rows quad_row and quad_row + 8.
+template <int NC>
+struct RowPair {
+    uint4 lo[NC], hi[NC];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) lo[i] = hi[i] = make_uint4(0, 0, 0, 0);
+    }
+};
+
+// d += A B for the two steps that one 16-byte chunk of every row makes.
+template <typename T>
+__device__ __forceinline__ void chunk_mma(float (&d)[4], const uint4& lo, const uint4& hi, const uint4& b) {
+    const uint32_t a0[4] = {lo.x, hi.x, lo.y, hi.y}, a1[4] = {lo.z, hi.z, lo.w, hi.w};
+    Mma<T>::run(d, a0, b.x, b.y);
+    Mma<T>::run(d, a1, b.z, b.w);
+}
+
+__device__ __forceinline__ const uint4* key_row(const WeighParams& p, const PageBounds& bounds, const uint32_t* row_ids,
+                                                uint32_t head, uint32_t key, uint32_t& bad) {
+    const uint32_t page = bounds.read(row_ids, key / p.geo.tokens_per_page, bad);
+    const uint64_t at = kv_row_offset(p.geo, page, head, key % p.geo.tokens_per_page);
+    return reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.geo.pages) + at);
+}
+
+__device__ __forceinline__ float* weight_row(const WeighParams& p, const WeighRequest& rq, uint32_t head) {
+    return p.weights + (uint64_t(rq.slot) * p.geo.num_kv_heads + head) * p.stride;
+}
+
+enum ShortMode { kStatsAndScores = 0, kStatsOnly = 1, kSumAgain = 2 };
+
+template <typename T, int NC, int kMode>
+__global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void weigh_short_kernel(const WeighParams p) {
+    await_previous_kernel();
+    const uint32_t count = p.scalars[kScalarWeighShort];
+    if (count == 0) return;
+    const WeighRequest* reqs = p.reqs;
+    const uint32_t total = reqs[count].cu0;
+    const uint32_t workers = min(gridDim.x * 8u, total);
+    const uint32_t w = blockIdx.x * 8u + (threadIdx.x >> 5);
+    if (w >= workers) return;
+    const uint32_t lane = threadIdx.x & 31u, quad_row = lane >> 2, quad_col = lane & 3u;
+    const uint32_t begin = uint32_t(uint64_t(w) * total / workers), end = uint32_t(uint64_t(w + 1) * total / workers);
+    const uint32_t chunks = p.geo.head_dim >> 3;
+    const PageBounds bounds(p.geo);
+    uint32_t bad = 0;
+    uint32_t r_index = find_request<0>(reqs, count, begin);
+    for (uint32_t tile = begin; tile < end;) {
+        while (reqs[r_index + 1].cu0 <= tile) ++r_index;
+        const WeighRequest rq = reqs[r_index];
+        const uint32_t per_head = (rq.keys + 31u) / 32u;
+        const uint32_t head = (tile - rq.cu0) / per_head;
+        const uint32_t unit_begin = rq.cu0 + head * per_head, unit_end = unit_begin + per_head;
+        const uint32_t last = min(end, unit_end);
+        const uint32_t rows = rq.q_len * p.group;
+        const uint32_t* row_ids = table_row(p.geo, rq.slot);
+        RowPair<NC> q;
+        q.zero();
+        if (quad_row < rows) load_row<NC>(q.lo, reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + query_row(p, rq, head, quad_row) * p.geo.head_dim), quad_col, chunks);
+        if (quad_row + 8 < rows) load_row<NC>(q.hi, reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + query_row(p, rq, head, quad_row + 8) * p.geo.head_dim), quad_col, chunks);
+        const uint32_t limit0 = quad_row < rows ? row_limit(p, rq, quad_row) : 0u;
+        const uint32_t limit1 = quad_row + 8 < rows ? row_limit(p, rq, quad_row + 8) : 0u;
+        Stat s0{-kInf, 0.0f}, s1{-kInf, 0.0f};
+        float lse0 = kInf, lse1 = kInf;
+        if (kMode == kSumAgain) {
+            if (quad_row < rows) lse0 = p.lse[query_row(p, rq, head, quad_row)];
+            if (quad_row + 8 < rows) lse1 = p.lse[query_row(p, rq, head, quad_row + 8)];
+        }
+        constexpr int kBatch = NC <= 4 ? 4 : 2;  // 8-key groups whose rows are in flight at once
+        for (; tile < last; ++tile) {
+            const uint32_t key0 = (tile - unit_begin) * 32u;
+#pragma unroll
+            for (int half = 0; half < 4; half += kBatch) {
+                uint4 k[kBatch][NC];
+#pragma unroll
+                for (int t = 0; t < kBatch; ++t) {
+                    const uint32_t key = min(key0 + 8u * (half + t) + quad_row, rq.keys - 1u);
+                    load_row<NC>(k[t], key_row(p, bounds, row_ids, head, key, bad), quad_col, chunks);
+                }
+                float s[kBatch][4];
+#pragma unroll
+                for (int t = 0; t < kBatch; ++t) {
+                    s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < NC; ++i) chunk_mma<T>(s[t], q.lo[i], q.hi[i], k[t][i]);
+                }
+#pragma unroll
+                for (int t = 0; t < kBatch; ++t) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t key = key0 + 8u * (half + t) + 2u * quad_col + (e & 1);
+                        s[t][e] = key < (e < 2 ? limit0 : limit1) ? s[t][e] * p.scale_log2 : -kInf;
+                    }
+                }
+                if (kMode == kSumAgain) {
+#pragma unroll
+                    for (int t = 0; t < kBatch; ++t) {
+                        float a = weight_of(s[t][0], lse0) + weight_of(s[t][2], lse1);
+                        float b = weight_of(s[t][1], lse0) + weight_of(s[t][3], lse1);
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) {
+                            a += __shfl_xor_sync(0xFFFFFFFFu, a, x);
+                            b += __shfl_xor_sync(0xFFFFFFFFu, b, x);
+                        }
+                        const uint32_t key = key0 + 8u * (half + t) + 2u * quad_col;
+                        float* row = weight_row(p, rq, head);
+                        if (quad_row == 0 && key < rq.keys) row[key] += a;
+                        if (quad_row == 0 && key + 1 < rq.keys) row[key + 1] += b;
+                    }
+                } else {
+                    if (kMode == kStatsAndScores) {
+#pragma unroll
+                        for (int t = 0; t < kBatch; ++t) {
+                            float* at = p.scores + (uint64_t(tile) * 4u + half + t) * 8u * p.score_rows + quad_row * 8u + 2u * quad_col;
+                            *reinterpret_cast<float2*>(at) = make_float2(s[t][0], s[t][1]);
+                            if (p.score_rows > 8) *reinterpret_cast<float2*>(at + 64) = make_float2(s[t][2], s[t][3]);
+                        }
+                    }
+                    float m0 = s0.m, m1 = s1.m;
+#pragma unroll
+                    for (int t = 0; t < kBatch; ++t) {
+                        m0 = fmaxf(m0, fmaxf(s[t][0], s[t][1]));
+                        m1 = fmaxf(m1, fmaxf(s[t][2], s[t][3]));
+                    }
+                    const float base0 = m0 == -kInf ? 0.0f : m0, base1 = m1 == -kInf ? 0.0f : m1;
+                    s0.l *= exp2f(s0.m - base0);
+                    s1.l *= exp2f(s1.m - base1);
+                    s0.m = m0;
+                    s1.m = m1;
+#pragma unroll
+                    for (int t = 0; t < kBatch; ++t) {
+                        s0.l += exp2f(s[t][0] - base0) + exp2f(s[t][1] - base0);
+                        s1.l += exp2f(s[t][2] - base1) + exp2f(s[t][3] - base1);
+                    }
+                }
+            }
+        }
+        if (kMode == kSumAgain) continue;
+#pragma unroll
+        for (int x = 1; x < 4; x <<= 1) {
+            s0.join(__shfl_xor_sync(0xFFFFFFFFu, s0.m, x), __shfl_xor_sync(0xFFFFFFFFu, s0.l, x));
+            s1.join(__shfl_xor_sync(0xFFFFFFFFu, s1.m, x), __shfl_xor_sync(0xFFFFFFFFu, s1.l, x));
+        }
+        // workers of this unit: the one that holds tile t is the last whose share begins at or before t
+        const uint32_t unit = r_index * p.geo.num_kv_heads + head;
+        const uint32_t first_worker = uint32_t((uint64_t(unit_begin + 1) * workers - 1) / total);
+        const uint32_t last_worker = uint32_t((uint64_t(unit_end) * workers - 1) / total);
+        if (first_worker == last_worker) {
+            if (quad_col == 0 && quad_row < rows) p.lse[query_row(p, rq, head, quad_row)] = s0.lse();
+            if (quad_col == 0 && quad_row + 8 < rows) p.lse[query_row(p, rq, head, quad_row + 8)] = s1.lse();
+            continue;
+        }
+        // worker + unit grows from one segment of the batch to the next: a slot of its own for each
+        float2* slot = p.partials + uint64_t(w + unit) * 16u;
+        if (quad_col == 0) {
+            slot[quad_row] = make_float2(s0.m, s0.l);
+            slot[quad_row + 8] = make_float2(s1.m, s1.l);
+        }
+        __threadfence();
+        __syncwarp();
+        uint32_t arrived = 0;
+        if (lane == 0) arrived = atomicAdd(p.counters + unit, 1u);
+        arrived = __shfl_sync(0xFFFFFFFFu, arrived, 0);
+        if (arrived == last_worker - first_worker) {
+            __threadfence();
+            Stat s{-kInf, 0.0f};
+            const uint32_t row = lane & 15u;
+            for (uint32_t o = first_worker + (lane >> 4); o <= last_worker; o += 2) {
+                const float2 v = __ldcg(p.partials + uint64_t(o + unit) * 16u + row);
+                s.join(v.x, v.y);
+            }
+            s.join(__shfl_xor_sync(0xFFFFFFFFu, s.m, 16), __shfl_xor_sync(0xFFFFFFFFu, s.l, 16));
+            if (lane < rows) p.lse[query_row(p, rq, head, lane)] = s.lse();
+            if (lane == 0) p.counters[unit] = 0;
+        }
+    }
+    if (bad != 0) record_page_fault(p.geo);
+}
+
+// Second pass over stored scores: a lane is a key.
+__global__ __launch_bounds__(256) void weigh_scores_kernel(const WeighParams p) {
+    await_previous_kernel();
+    const uint32_t count = p.scalars[kScalarWeighShort];
+    if (count == 0) return;
+    const WeighRequest* reqs = p.reqs;
+    const uint32_t total = reqs[count].cu0;
+    const uint32_t workers = min(gridDim.x * 8u, total);
+    const uint32_t w = blockIdx.x * 8u + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
+    if (w >= workers) return;
+    const uint32_t begin = uint32_t(uint64_t(w) * total / workers), end = uint32_t(uint64_t(w + 1) * total / workers);
+    uint32_t r_index = find_request<0>(reqs, count, begin);
+    for (uint32_t tile = begin; tile < end; ++tile) {
+        while (reqs[r_index + 1].cu0 <= tile) ++r_index;
+        const WeighRequest rq = reqs[r_index];
+        const uint32_t per_head = (rq.keys + 31u) / 32u;
+        const uint32_t head = (tile - rq.cu0) / per_head;
+        const uint32_t key = (tile - rq.cu0 - head * per_head) * 32u + lane;
+        const uint32_t rows = rq.q_len * p.group;
+        const float* s = p.scores + (uint64_t(tile) * 4u + (lane >> 3)) * 8u * p.score_rows + (lane & 7u);
+        float sum = 0.0f;
+        for (uint32_t r = 0; r < rows; ++r) sum += weight_of(s[r * 8u], p.lse[query_row(p, rq, head, r)]);
+        if (key < rq.keys) weight_row(p, rq, head)[key] += sum;
+    }
+}
+
+// ---- runs of more than 16 rows -------------------------------------------------------------------------------------------
+
+constexpr uint32_t kBlock = kWeighBlock;  // rows or keys of one A block, and of one B block
+
+// Byte offset of 16-byte chunk `chunk` of row `row` in a B block of NC * 64-byte rows: the eight lanes of one phase of a
+// 16-byte read (two rows, four chunks) fall into distinct banks.
+template <int NC>
+__device__ __forceinline__ uint32_t block_offset(uint32_t row, uint32_t chunk) {
+    return row * (NC * 64u) + ((NC % 2 == 0 ? chunk ^ ((row & 1u) << 2) : chunk) << 4);
+}
+
+// The 64 x 64 product of a warp's 16 A rows and the B block in shared memory.
+template <typename T, int NC>
+__device__ __forceinline__ void block_product(float (&s)[8][4], const RowPair<NC>& a, const unsigned char* b, uint32_t quad_row,
+                                              uint32_t quad_col) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            const uint4 v = *reinterpret_cast<const uint4*>(b + block_offset<NC>(8u * t + quad_row, quad_col + 4u * i));
+            chunk_mma<T>(s[t], a.lo[i], a.hi[i], v);
+        }
+    }
+}
+
+template <int NC>
+__device__ __forceinline__ void copy_row(uint32_t smem, uint32_t row, const uint4* src, bool live, uint32_t chunks) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const uint32_t c = (threadIdx.x & 3u) + 4u * i;
+        cp_async_16(smem + block_offset<NC>(row, c), src + (c < chunks ? c : 0u), live && c < chunks ? 16u : 0u);
+    }
+}
+
+// First pass: item = (request, KV head, 64 rows, piece of the keys).
+template <typename T, int NC>
+__global__ __launch_bounds__(128) void weigh_stats_kernel(const WeighParams p) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ uint32_t last_arrival;
+    await_previous_kernel();
+    const uint32_t count = p.scalars[kScalarWeighLong];
+    if (count == 0) return;
+    const WeighRequest* reqs = p.long_reqs();
+    const uint32_t total = reqs[count].cu0;
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, quad_row = lane >> 2, quad_col = lane & 3u;
+    const uint32_t chunks = p.geo.head_dim >> 3;
+    const uint32_t smem_base = uint32_t(__cvta_generic_to_shared(smem));
+    const PageBounds bounds(p.geo);
+    uint32_t bad = 0;
+    for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
+        const uint32_t r_index = find_request<0>(reqs, count, item);
+        const WeighRequest rq = reqs[r_index];
+        const uint32_t pieces = weigh_pieces(rq.keys), rows = rq.q_len * p.group, blocks = (rows + kBlock - 1) / kBlock;
+        const uint32_t local = item - rq.cu0, piece = local % pieces, unit = local / pieces;
+        const uint32_t head = unit / blocks, row0 = (unit % blocks) * kBlock;
+        const uint32_t piece_keys = weigh_piece_keys(rq.keys, pieces);
+        const uint32_t seen = row_limit(p, rq, min(row0 + kBlock, rows) - 1);
+        const uint32_t k0 = piece * piece_keys, k1 = min(min(k0 + piece_keys, rq.keys), seen);
+        const uint32_t* row_ids = table_row(p.geo, rq.slot);
+        const uint32_t ra = row0 + warp * 16u + quad_row, rb = ra + 8u;
+        const uint32_t limit0 = ra < rows ? row_limit(p, rq, ra) : 0u, limit1 = rb < rows ? row_limit(p, rq, rb) : 0u;
+        Stat s0{-kInf, 0.0f}, s1{-kInf, 0.0f};
+        if (k0 < k1) {
+            RowPair<NC> q;
+            q.zero();
+            if (ra < rows) load_row<NC>(q.lo, reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + query_row(p, rq, head, ra) * p.geo.head_dim), quad_col, chunks);
+            if (rb < rows) load_row<NC>(q.hi, reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + query_row(p, rq, head, rb) * p.geo.head_dim), quad_col, chunks);
+            const auto fetch = [&](uint32_t key0, uint32_t stage) {
+#pragma unroll
+                for (uint32_t half = 0; half < 2; ++half) {
+                    const uint32_t row = (threadIdx.x >> 2) + 32u * half, key = key0 + row;
+                    copy_row<NC>(smem_base + stage * (kBlock * NC * 64u), row, key_row(p, bounds, row_ids, head, min(key, k1 - 1), bad), key < k1, chunks);
+                }
+                cp_async_commit();
+            };
+            fetch(k0, 0);
+            uint32_t stage = 0;
+            for (uint32_t key0 = k0; key0 < k1; key0 += kBlock, stage ^= 1u) {
+                if (key0 + kBlock < k1) {
+                    fetch(key0 + kBlock, stage ^ 1u);
+                    cp_async_wait<1>();
+                } else {
+                    cp_async_wait<0>();
+                }
+                __syncthreads();
+                float s[8][4];
+                block_product<T, NC>(s, q, smem + stage * (kBlock * NC * 64u), quad_row, quad_col);
+                float m0 = s0.m, m1 = s1.m;
+#pragma unroll
+                for (int t = 0; t < 8; ++t) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t key = key0 + 8u * t + 2u * quad_col + (e & 1);
+                        s[t][e] = key < min(k1, e < 2 ? limit0 : limit1) ? s[t][e] * p.scale_log2 : -kInf;
+                    }
+                    m0 = fmaxf(m0, fmaxf(s[t][0], s[t][1]));
+                    m1 = fmaxf(m1, fmaxf(s[t][2], s[t][3]));
+                }
+                const float base0 = m0 == -kInf ? 0.0f : m0, base1 = m1 == -kInf ? 0.0f : m1;
+                s0.l *= exp2f(s0.m - base0);
+                s1.l *= exp2f(s1.m - base1);
+                s0.m = m0;
+                s1.m = m1;
+#pragma unroll
+                for (int t = 0; t < 8; ++t) {
+                    s0.l += exp2f(s[t][0] - base0) + exp2f(s[t][1] - base0);
+                    s1.l += exp2f(s[t][2] - base1) + exp2f(s[t][3] - base1);
+                }
+                __syncthreads();
+            }
+#pragma unroll
+            for (int x = 1; x < 4; x <<= 1) {
+                s0.join(__shfl_xor_sync(0xFFFFFFFFu, s0.m, x), __shfl_xor_sync(0xFFFFFFFFu, s0.l, x));
+                s1.join(__shfl_xor_sync(0xFFFFFFFFu, s1.m, x), __shfl_xor_sync(0xFFFFFFFFu, s1.l, x));
+            }
+        }
+        if (pieces == 1) {
+            if (quad_col == 0 && ra < rows) p.lse[query_row(p, rq, head, ra)] = s0.lse();
+            if (quad_col == 0 && rb < rows) p.lse[query_row(p, rq, head, rb)] = s1.lse();
+            continue;
+        }
+        float2* slot = p.long_partials() + uint64_t(item) * kBlock;
+        if (quad_col == 0) {
+            slot[warp * 16u + quad_row] = make_float2(s0.m, s0.l);
+            slot[warp * 16u + quad_row + 8u] = make_float2(s1.m, s1.l);
+        }
+        __threadfence();
+        __syncthreads();
+        uint32_t* counter = p.long_counters() + rq.unit0 + unit;
+        if (threadIdx.x == 0) last_arrival = atomicAdd(counter, 1u) == pieces - 1 ? 1u : 0u;
+        __syncthreads();
+        if (last_arrival != 0) {
+            __threadfence();
+            const uint32_t row = row0 + threadIdx.x;
+            if (threadIdx.x < kBlock && row < rows) {
+                Stat s{-kInf, 0.0f};
+                for (uint32_t o = 0; o < pieces; ++o) {
+                    const float2 v = __ldcg(p.long_partials() + uint64_t(rq.cu0 + unit * pieces + o) * kBlock + threadIdx.x);
+                    s.join(v.x, v.y);
+                }
+                p.lse[query_row(p, rq, head, row)] = s.lse();
+            }
+            if (threadIdx.x == 0) *counter = 0;
+        }
+        __syncthreads();
+    }
+    if (bad != 0) record_page_fault(p.geo);
+}
+
+// Second pass: item = (request, KV head, 64 keys); the request's rows pass by in blocks of 64.
+template <typename T, int NC>
+__global__ __launch_bounds__(128) void weigh_sum_kernel(const WeighParams p) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float lse[2][kBlock];
+    await_previous_kernel();
+    const uint32_t count = p.scalars[kScalarWeighLong];
+    if (count == 0) return;
+    const WeighRequest* reqs = p.long_reqs();
+    const uint32_t total = reqs[count].cu1;
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, quad_row = lane >> 2, quad_col = lane & 3u;
+    const uint32_t chunks = p.geo.head_dim >> 3;
+    const uint32_t smem_base = uint32_t(__cvta_generic_to_shared(smem));
+    const PageBounds bounds(p.geo);
+    uint32_t bad = 0;
+    for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
+        const uint32_t r_index = find_request<1>(reqs, count, item);
+        const WeighRequest rq = reqs[r_index];
+        const uint32_t rows = rq.q_len * p.group, key_blocks = (rq.keys + kBlock - 1) / kBlock;
+        const uint32_t head = (item - rq.cu1) / key_blocks, key0 = (item - rq.cu1) % key_blocks * kBlock;
+        const uint32_t* row_ids = table_row(p.geo, rq.slot);
+        const uint32_t ka = key0 + warp * 16u + quad_row, kb = ka + 8u;
+        RowPair<NC> k;
+        load_row<NC>(k.lo, key_row(p, bounds, row_ids, head, min(ka, rq.keys - 1), bad), quad_col, chunks);
+        load_row<NC>(k.hi, key_row(p, bounds, row_ids, head, min(kb, rq.keys - 1), bad), quad_col, chunks);
+        // rows of tokens before the block's first key see none of it
+        const uint32_t row_begin = key0 > rq.first_pos ? (key0 - rq.first_pos) * p.group : 0u;
+        const auto fetch = [&](uint32_t row0, uint32_t stage) {
+#pragma unroll
+            for (uint32_t half = 0; half < 2; ++half) {
+                const uint32_t at = (threadIdx.x >> 2) + 32u * half, row = row0 + at;
+                const uint64_t q_row = query_row(p, rq, head, min(row, rows - 1));
+                copy_row<NC>(smem_base + stage * (kBlock * NC * 64u), at,
+                             reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + q_row * p.geo.head_dim), row < rows, chunks);
+                if ((threadIdx.x & 3u) == 0) lse[stage][at] = row < rows ? p.lse[q_row] : kInf;
+            }
+            cp_async_commit();
+        };
+        float sum0 = 0.0f, sum1 = 0.0f;
+        if (row_begin < rows) fetch(row_begin, 0);
+        uint32_t stage = 0;
+        for (uint32_t row0 = row_begin; row0 < rows; row0 += kBlock, stage ^= 1u) {
+            if (row0 + kBlock < rows) {
+                fetch(row0 + kBlock, stage ^ 1u);
+                cp_async_wait<1>();
+            } else {
+                cp_async_wait<0>();
+            }
+            __syncthreads();
+            float s[8][4];
+            block_product<T, NC>(s, k, smem + stage * (kBlock * NC * 64u), quad_row, quad_col);
+            const bool masked = key0 + kBlock > row_limit(p, rq, row0);
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                const float2 n = *reinterpret_cast<const float2*>(&lse[stage][8 * t + 2 * quad_col]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float w = weight_of(s[t][e] * p.scale_log2, e & 1 ? n.y : n.x);
+                    if (masked && (e < 2 ? ka : kb) >= row_limit(p, rq, row0 + 8u * t + 2u * quad_col + (e & 1))) w = 0.0f;
+                    if (e < 2) sum0 += w;
+                    else sum1 += w;
+                }
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int x = 1; x < 4; x <<= 1) {
+            sum0 += __shfl_xor_sync(0xFFFFFFFFu, sum0, x);
+            sum1 += __shfl_xor_sync(0xFFFFFFFFu, sum1, x);
+        }
+        float* out = weight_row(p, rq, head);
+        if (quad_col == 0 && ka < rq.keys) out[ka] += sum0;
+        if (quad_col == 0 && kb < rq.keys) out[kb] += sum1;
+    }
+    if (bad != 0) record_page_fault(p.geo);
+}
+
+// ---- any type and head_dim: f32 products on the CUDA cores, 16 rows against 64 keys -----------------------------------------
+
+constexpr uint32_t kAnyRows = kWeighAnyRows;
+
+struct AnyTile {
+    float* q;  // [16][d]
+    float* k;  // [64][d + 1]
+    uint32_t d;
+    __device__ __forceinline__ AnyTile(float* smem, uint32_t head_dim) : q(smem), k(smem + kAnyRows * head_dim), d(head_dim) {}
+    __device__ __forceinline__ void load_rows(const WeighParams& p, const WeighRequest& rq, uint32_t head, uint32_t row0, uint32_t rows) {
+        for (uint32_t i = threadIdx.x; i < kAnyRows * d; i += blockDim.x) {
+            const uint32_t row = row0 + i / d;
+            q[i] = row < rows ? load_as_float(p.q, query_row(p, rq, head, row) * d + i % d, p.dtype) : 0.0f;
+        }
+    }
+    __device__ __forceinline__ void load_keys(const WeighParams& p, const PageBounds& bounds, const uint32_t* row_ids, uint32_t head,
+                                              uint32_t key0, uint32_t keys, uint32_t& bad) {
+        for (uint32_t at = threadIdx.x >> 5; at < kBlock; at += blockDim.x >> 5) {
+            const uint32_t key = key0 + at;
+            if (key >= keys) continue;  // never read: those columns are masked
+            const uint32_t page = bounds.read(row_ids, key / p.geo.tokens_per_page, bad);
+            const uint64_t row = kv_row_offset(p.geo, page, head, key % p.geo.tokens_per_page);
+            for (uint32_t i = threadIdx.x & 31u; i < d; i += 32u) k[at * (d + 1) + i] = load_as_float(p.geo.pages, row + i, p.dtype);
+        }
+    }
+    // Thread t: rows 2 (t / 16) + {0, 1}, keys t % 16 + 16 {0..3}.
+    __device__ __forceinline__ void product(float (&s)[2][4]) const {
+        const uint32_t row = 2u * (threadIdx.x >> 4), key = threadIdx.x & 15u;
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) s[a][b] = 0.0f;
+        for (uint32_t i = 0; i < d; ++i) {
+            const float q0 = q[row * d + i], q1 = q[(row + 1) * d + i];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const float x = k[(key + 16u * b) * (d + 1) + i];
+                s[0][b] = fmaf(q0, x, s[0][b]);
+                s[1][b] = fmaf(q1, x, s[1][b]);
+            }
+        }
+    }
+};
+
+__global__ __launch_bounds__(128) void weigh_stats_any_kernel(const WeighParams p) {
+    extern __shared__ __align__(16) float any_smem[];
+    __shared__ uint32_t last_arrival;
+    await_previous_kernel();
+    const uint32_t count = p.scalars[kScalarWeighLong];
+    if (count == 0) return;
+    const WeighRequest* reqs = p.long_reqs();
+    const uint32_t total = reqs[count].cu0;
+    const PageBounds bounds(p.geo);
+    uint32_t bad = 0;
+    AnyTile tile(any_smem, p.geo.head_dim);
+    const uint32_t at = 2u * (threadIdx.x >> 4), column = threadIdx.x & 15u;
+    for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
+        const WeighRequest rq = reqs[find_request<0>(reqs, count, item)];
+        const uint32_t pieces = weigh_pieces(rq.keys), rows = rq.q_len * p.group, blocks = (rows + kAnyRows - 1) / kAnyRows;
+        const uint32_t local = item - rq.cu0, piece = local % pieces, unit = local / pieces;
+        const uint32_t head = unit / blocks, row0 = (unit % blocks) * kAnyRows;
+        const uint32_t piece_keys = weigh_piece_keys(rq.keys, pieces);
+        const uint32_t k0 = piece * piece_keys;
+        const uint32_t k1 = min(min(k0 + piece_keys, rq.keys), row_limit(p, rq, min(row0 + kAnyRows, rows) - 1));
+        const uint32_t* row_ids = table_row(p.geo, rq.slot);
+        Stat st[2] = {{-kInf, 0.0f}, {-kInf, 0.0f}};
+        tile.load_rows(p, rq, head, row0, rows);
+        for (uint32_t key0 = k0; key0 < k1; key0 += kBlock) {
+            tile.load_keys(p, bounds, row_ids, head, key0, k1, bad);
+            __syncthreads();
+            float s[2][4];
+            tile.product(s);
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                const uint32_t row = row0 + at + a, limit = row < rows ? min(k1, row_limit(p, rq, row)) : 0u;
+                float m = st[a].m;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    s[a][b] = key0 + column + 16u * b < limit ? s[a][b] * p.scale_log2 : -kInf;
+                    m = fmaxf(m, s[a][b]);
+                }
+                const float base = m == -kInf ? 0.0f : m;
+                st[a].l *= exp2f(st[a].m - base);
+                st[a].m = m;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) st[a].l += exp2f(s[a][b] - base);
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int x = 1; x < 16; x <<= 1)
+                st[a].join(__shfl_xor_sync(0xFFFFFFFFu, st[a].m, x), __shfl_xor_sync(0xFFFFFFFFu, st[a].l, x));
+        if (column == 0) {
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                if (pieces == 1) {
+                    if (row0 + at + a < rows) p.lse[query_row(p, rq, head, row0 + at + a)] = st[a].lse();
+                } else {
+                    p.long_partials()[uint64_t(item) * kAnyRows + at + a] = make_float2(st[a].m, st[a].l);
+                }
+            }
+        }
+        if (pieces > 1) {
+            uint32_t* counter = p.long_counters() + rq.unit0 + unit;
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) last_arrival = atomicAdd(counter, 1u) == pieces - 1 ? 1u : 0u;
+            __syncthreads();
+            if (last_arrival != 0) {
+                __threadfence();
+                const uint32_t row = row0 + threadIdx.x;
+                if (threadIdx.x < kAnyRows && row < rows) {
+                    Stat s{-kInf, 0.0f};
+                    for (uint32_t o = 0; o < pieces; ++o) {
+                        const float2 v = __ldcg(p.long_partials() + uint64_t(rq.cu0 + unit * pieces + o) * kAnyRows + threadIdx.x);
+                        s.join(v.x, v.y);
+                    }
+                    p.lse[query_row(p, rq, head, row)] = s.lse();
+                }
+                if (threadIdx.x == 0) *counter = 0;
+            }
+        }
+        __syncthreads();
+    }
+    if (bad != 0) record_page_fault(p.geo);
+}
+
+__global__ __launch_bounds__(128) void weigh_sum_any_kernel(const WeighParams p) {
+    extern __shared__ __align__(16) float any_smem[];
+    __shared__ float sums[8][kBlock];
+    __shared__ float lse[kAnyRows];
+    await_previous_kernel();
+    const uint32_t count = p.scalars[kScalarWeighLong];
+    if (count == 0) return;
+    const WeighRequest* reqs = p.long_reqs();
+    const uint32_t total = reqs[count].cu1;
+    const PageBounds bounds(p.geo);
+    uint32_t bad = 0;
+    AnyTile tile(any_smem, p.geo.head_dim);
+    const uint32_t at = 2u * (threadIdx.x >> 4), column = threadIdx.x & 15u;
+    for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
+        const WeighRequest rq = reqs[find_request<1>(reqs, count, item)];
+        const uint32_t rows = rq.q_len * p.group, key_blocks = (rq.keys + kBlock - 1) / kBlock;
+        const uint32_t head = (item - rq.cu1) / key_blocks, key0 = (item - rq.cu1) % key_blocks * kBlock;
+        const uint32_t row_begin = key0 > rq.first_pos ? (key0 - rq.first_pos) * p.group : 0u;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        tile.load_keys(p, bounds, table_row(p.geo, rq.slot), head, key0, rq.keys, bad);
+        for (uint32_t row0 = row_begin; row0 < rows; row0 += kAnyRows) {
+            tile.load_rows(p, rq, head, row0, rows);
+            if (threadIdx.x < kAnyRows) lse[threadIdx.x] = row0 + threadIdx.x < rows ? p.lse[query_row(p, rq, head, row0 + threadIdx.x)] : kInf;
+            __syncthreads();
+            float s[2][4];
+            tile.product(s);
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                const uint32_t row = row0 + at + a, limit = row < rows ? row_limit(p, rq, row) : 0u;
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                    if (key0 + column + 16u * b < limit) sum[b] += weight_of(s[a][b] * p.scale_log2, lse[at + a]);
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) sums[threadIdx.x >> 4][column + 16u * b] = sum[b];
+        __syncthreads();
+        if (threadIdx.x < kBlock && key0 + threadIdx.x < rq.keys) {
+            float all = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) all += sums[i][threadIdx.x];
+            weight_row(p, rq, head)[key0 + threadIdx.x] += all;
+        }
+        __syncthreads();
+    }
+    if (bad != 0) record_page_fault(p.geo);
+}
+
+template <typename T, int NC, int kMode>
+cudaError_t launch_short(const WeighParams& p, uint32_t ctas, cudaStream_t stream) {
+    return launch_overlapped(weigh_short_kernel<T, NC, kMode>, dim3(ctas), dim3(256), 0, stream, p);
+}
+
+template <typename T, int NC>
+cudaError_t launch_tensor(const WeighParams& p, WeighPass pass, uint32_t ctas, cudaStream_t stream) {
+    constexpr int kSmem = 2 * kBlock * NC * 64;
+    switch (pass) {
+        case WeighPass::kShortStatsScores: return launch_short<T, NC, kStatsAndScores>(p, ctas, stream);
+        case WeighPass::kShortStats: return launch_short<T, NC, kStatsOnly>(p, ctas, stream);
+        case WeighPass::kShortSumAgain: return launch_short<T, NC, kSumAgain>(p, ctas, stream);
+        case WeighPass::kLongStats: {
+            static std::atomic<uint64_t> done{0};
+            const cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(weigh_stats_kernel<T, NC>), kSmem, done);
+            if (err != cudaSuccess) return err;
+            return launch_overlapped(weigh_stats_kernel<T, NC>, dim3(ctas), dim3(128), kSmem, stream, p);
+        }
+        case WeighPass::kLongSum: {
+            static std::atomic<uint64_t> done{0};
+            const cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(weigh_sum_kernel<T, NC>), kSmem, done);
+            if (err != cudaSuccess) return err;
+            return launch_overlapped(weigh_sum_kernel<T, NC>, dim3(ctas), dim3(128), kSmem, stream, p);
+        }
+        default: return cudaErrorInvalidValue;
+    }
+}
+
+template <typename T>
+cudaError_t launch_typed(const WeighParams& p, WeighPass pass, uint32_t ctas, cudaStream_t stream) {
+    const uint32_t d = p.geo.head_dim;  // 64-byte pieces of a row, rounded up to a compiled count
+    if (d <= 64) return launch_tensor<T, 2>(p, pass, ctas, stream);
+    if (d <= 96) return launch_tensor<T, 3>(p, pass, ctas, stream);
+    if (d <= 128) return launch_tensor<T, 4>(p, pass, ctas, stream);
+    if (d <= 192) return launch_tensor<T, 6>(p, pass, ctas, stream);
+    return launch_tensor<T, 8>(p, pass, ctas, stream);
+}
+
+cudaError_t launch_any(const WeighParams& p, WeighPass pass, uint32_t ctas, cudaStream_t stream) {
+    const int most = int((kAnyRows * 256 + kBlock * 257) * sizeof(float));
+    const size_t smem = (kAnyRows * p.geo.head_dim + kBlock * (p.geo.head_dim + 1)) * sizeof(float);
+    static std::atomic<uint64_t> stats_done{0}, sum_done{0};
+    const bool stats = pass == WeighPass::kLongStats;
+    const cudaError_t err = stats ? ensure_dynamic_smem(reinterpret_cast<const void*>(weigh_stats_any_kernel), most, stats_done)
+                                  : ensure_dynamic_smem(reinterpret_cast<const void*>(weigh_sum_any_kernel), most, sum_done);
+    if (err != cudaSuccess) return err;
+    return launch_overlapped(stats ? weigh_stats_any_kernel : weigh_sum_any_kernel, dim3(ctas), dim3(128), smem, stream, p);
+}
+
+}  // namespace
+
+cudaError_t launch_weigh(const WeighParams& p, WeighPass pass, uint32_t ctas, cudaStream_t stream) {
+    if (pass == WeighPass::kShortSumScores) return launch_overlapped(weigh_scores_kernel, dim3(ctas), dim3(256), 0, stream, p);
+    if (!weigh_on_tensor_cores(p.dtype, p.geo.head_dim)) return launch_any(p, pass, ctas, stream);
+    return p.dtype == PSI_DTYPE_BF16 ? launch_typed<__nv_bfloat16>(p, pass, ctas, stream) : launch_typed<__half>(p, pass, ctas, stream);
+}
+
+}  // namespace psi
