@@ -647,6 +647,8 @@ PSI_API int32_t psi_linear_prepare(psi_linear* linear, const uint32_t* req_slots
  * request.  The same call gives the same bits.  May be captured: a replay takes the batch prepared last. */
 PSI_API int32_t psi_linear_attend(psi_linear* linear, uint32_t layer, float* states, const void* q, const void* k, const void* v,
                                   void* out);
+/* As psi_gqa_device_status: waits for the stream; PSI_ERR_TIMEOUT when a bounded wait of a launch gave up. */
+PSI_API int32_t psi_linear_device_status(psi_linear* linear, int32_t* out);
 
 /* Number of kernels this library has launched on the context since creation (for launch accounting). */
 PSI_API int32_t psi_ctx_launch_count(psi_ctx* ctx, uint64_t* out);

@@ -763,6 +763,12 @@ class LinearAttention:
         _check(library().psi_linear_attend(self._h, C.c_uint32(layer), _ptr(states), _ptr(q), _ptr(k), _ptr(v), _ptr(out)),
                self.ctx._h)
 
+    def device_status(self) -> int:
+        """Waits for the stream; returns 0, or the status a bounded device-side wait recorded (4 = timeout)."""
+        out = C.c_int32()
+        _check(library().psi_linear_device_status(self._h, C.byref(out)), self.ctx._h)
+        return out.value
+
 
 def attend_static(device, stream, config: GQAConfig, pages, page_table, req_slots, token_indices, cu_tokens, layer, q,
                   out):

@@ -11,12 +11,25 @@ struct psi_linear {
     uint32_t* staging = nullptr;
     cudaEvent_t upload_done = nullptr;
     DeviceBuffer decays;       // [layers][Hv][kLinearDecays]
-    uint32_t num_steps = 0;    // requests of the prepared batch
+    DeviceBuffer status_word;  // u32 written by bounded device-side waits
+    bool chunked = false;      // long runs take the chunked form
+    uint32_t num_steps = 0, num_runs = 0;  // of the prepared batch
     bool prepared = false;
     std::vector<uint32_t> reads, writes;  // by slot: readers of it in the batch at hand, and whether one writes it
 };
 
 namespace {
+
+// Runs of more tokens take the chunked form.
+constexpr uint32_t kStepTokens = 16;
+
+// What the kernels know of a head's decay (kLinearDecays).
+void fill_decay(float* out, float log_decay) {
+    for (uint32_t i = 0; i <= kLinearChunk; ++i) out[i] = float(std::exp(double(log_decay) * i));
+    out[kLinearChunkLow] = float(std::exp(double(log_decay) * kLinearChunk) - double(out[kLinearChunk]));
+    out[kLinearStepLow] = float(std::exp(double(log_decay)) - double(out[1]));
+    out[kLinearStepLow + 1] = 0.0f;
+}
 
 uint64_t block_capacity(const psi_linear* l) { return kLinearScalarCount + uint64_t(l->cfg.max_tokens) * kLinearRequestWords; }
 
@@ -47,10 +60,12 @@ int32_t psi_linear_create(psi_ctx* ctx, const psi_linear_config* config, psi_lin
         l->reads.assign(c.num_req_slots, 0);
         l->writes.assign(c.num_req_slots, 0);
         const uint64_t decays = uint64_t(c.num_layers) * c.num_v_heads;
-        std::vector<float> none(decays * kLinearDecays, 0.0f);  // lambda = 1
-        for (uint64_t i = 0; i < decays; ++i) none[i * kLinearDecays] = 1.0f;
+        std::vector<float> none(decays * kLinearDecays);
+        for (uint64_t i = 0; i < decays; ++i) fill_decay(none.data() + i * kLinearDecays, 0.0f);
+        l->chunked = linear_chunk_supported(c.dtype, c.key_dim, c.value_dim) && c.max_tokens > kStepTokens;
         try {
             l->block.ensure(ctx, block_capacity(l.get()) * sizeof(uint32_t), true);
+            l->status_word.ensure(ctx, sizeof(uint32_t), true);
             l->decays.ensure(ctx, none.size() * sizeof(float), false);
             cuda_check(cudaMemcpyAsync(l->decays.ptr, none.data(), none.size() * sizeof(float), cudaMemcpyHostToDevice, ctx->stream),
                        "cudaMemcpyAsync");  // pageable source: staged before the call returns
@@ -59,6 +74,7 @@ int32_t psi_linear_create(psi_ctx* ctx, const psi_linear_config* config, psi_lin
         } catch (...) {
             l->block.release();
             l->decays.release();
+            l->status_word.release();
             if (l->staging != nullptr) (void)cudaFreeHost(l->staging);
             throw;
         }
@@ -73,6 +89,7 @@ int32_t psi_linear_destroy(psi_linear* l) {
         (void)cudaStreamSynchronize(l->ctx->stream);
         l->block.release();
         l->decays.release();
+        l->status_word.release();
         if (l->staging != nullptr) (void)cudaFreeHost(l->staging);
         if (l->upload_done != nullptr) (void)cudaEventDestroy(l->upload_done);
     });
@@ -91,10 +108,7 @@ int32_t psi_linear_set_decay(psi_linear* l, uint32_t layer, const float* log_dec
         std::vector<float> parts(uint64_t(heads) * kLinearDecays);
         for (uint32_t h = 0; h < heads; ++h) {
             require(std::isfinite(log_decay[h]) && log_decay[h] <= 0.0f, "log_decay must be finite and not positive");
-            const double lambda = std::exp(double(log_decay[h]));
-            parts[h * kLinearDecays] = float(lambda);
-            parts[h * kLinearDecays + 1] = float(lambda - double(float(lambda)));
-            parts[h * kLinearDecays + 2] = log_decay[h];
+            fill_decay(parts.data() + uint64_t(h) * kLinearDecays, log_decay[h]);
         }
         ctx->bind();
         cuda_check(cudaMemcpyAsync(static_cast<float*>(l->decays.ptr) + uint64_t(layer) * heads * kLinearDecays, parts.data(),
@@ -141,14 +155,24 @@ int32_t psi_linear_prepare(psi_linear* l, const uint32_t* req_slots, const uint3
         uint32_t n = 0;
         for (uint32_t r = 0; r < num_reqs; ++r) {
             const uint32_t q_len = cu_tokens[r + 1] - cu_tokens[r];
-            if (q_len > 0) reqs[n++] = LinearRequest{req_slots[r], outs[r], token_indices[r] == 0 ? 1u : 0u, q_len, cu_tokens[r], {0, 0, 0}};
+            if (q_len > 0 && !(l->chunked && q_len > kStepTokens))
+                reqs[n++] = LinearRequest{req_slots[r], outs[r], token_indices[r] == 0 ? 1u : 0u, q_len, cu_tokens[r], {0, 0, 0}};
         }
+        l->num_steps = n;
+        auto* runs = reinterpret_cast<LinearRun*>(reqs + n);
+        uint32_t num_runs = 0;
+        for (uint32_t r = 0; r < num_reqs && l->chunked; ++r) {
+            const uint32_t q_len = cu_tokens[r + 1] - cu_tokens[r];
+            if (q_len > kStepTokens)
+                runs[num_runs++] = LinearRun{req_slots[r], outs[r], token_indices[r] == 0 ? 1u : 0u, 1, cu_tokens[r], q_len, kLinearNoCarry, kLinearNoCarry};
+        }
+        l->num_runs = num_runs;
         l->staging[kLinearNumSteps] = n;
-        cuda_check(cudaMemcpyAsync(l->block.ptr, l->staging, (kLinearScalarCount + n * kLinearRequestWords) * sizeof(uint32_t),
+        l->staging[kLinearNumRuns] = num_runs;
+        cuda_check(cudaMemcpyAsync(l->block.ptr, l->staging, (kLinearScalarCount + (n + num_runs) * kLinearRequestWords) * sizeof(uint32_t),
                                    cudaMemcpyHostToDevice, ctx->stream),
                    "cudaMemcpyAsync");
         cuda_check(cudaEventRecord(l->upload_done, ctx->stream), "cudaEventRecord");
-        l->num_steps = n;
         l->prepared = true;
     });
 }
@@ -166,6 +190,7 @@ int32_t psi_linear_attend(psi_linear* l, uint32_t layer, float* states, const vo
                 "linear attention buffers must be aligned to their elements");
         ctx->bind();
         LinearParams p{};
+        p.status = static_cast<uint32_t*>(l->status_word.ptr);
         p.scalars = static_cast<const uint32_t*>(l->block.ptr);
         p.reqs = reinterpret_cast<const LinearRequest*>(p.scalars + kLinearScalarCount);
         p.decays = static_cast<const float*>(l->decays.ptr) + uint64_t(layer) * l->cfg.num_v_heads * kLinearDecays;
@@ -182,12 +207,33 @@ int32_t psi_linear_attend(psi_linear* l, uint32_t layer, float* states, const vo
         p.value_dim = l->cfg.value_dim;
         p.dtype = l->cfg.dtype;
         p.scale = l->cfg.scale;
+        p.aligned = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0 ? 1u : 0u;
         const uint64_t wave = static_cast<uint64_t>(ctx->sm_count) * 16;
         const uint64_t per_request = uint64_t(l->cfg.num_v_heads) * linear_step_slices(l->cfg.value_dim);
         // a captured launch has to be right for every later batch: its grid does not depend on this one
         const uint64_t items = (ctx->capturing ? uint64_t(l->cfg.max_tokens) : l->num_steps) * per_request;
-        LaunchScope scope(ctx, PSI_KERNEL_CLASS_LINEAR);
-        cuda_check(launch_linear_step(p, static_cast<uint32_t>(std::min(items, wave)), ctx->stream), "linear attention launch");
+        if (items > 0) {
+            LaunchScope scope(ctx, PSI_KERNEL_CLASS_LINEAR);
+            cuda_check(launch_linear_step(p, static_cast<uint32_t>(std::min(items, wave)), ctx->stream), "linear attention launch");
+        }
+        const uint64_t sms = static_cast<uint64_t>(ctx->sm_count);
+        const uint64_t run_items = !l->chunked ? 0 : ctx->capturing ? sms : uint64_t(l->num_runs) * l->cfg.num_v_heads;
+        if (run_items > 0) {
+            LaunchScope scope(ctx, PSI_KERNEL_CLASS_LINEAR);
+            cuda_check(launch_linear_chunk(p, false, static_cast<uint32_t>(std::min(run_items, sms)), ctx->stream), "linear attention (chunk) launch");
+        }
+    });
+}
+
+int32_t psi_linear_device_status(psi_linear* l, int32_t* out) {
+    if (l == nullptr || out == nullptr) return PSI_ERR_INVALID_ARGUMENT;
+    return guarded(l->ctx, [&] {
+        l->ctx->bind();
+        cuda_check(cudaStreamSynchronize(l->ctx->stream), "cudaStreamSynchronize");
+        uint32_t word = 0;
+        cuda_check(cudaMemcpy(&word, l->status_word.ptr, sizeof(word), cudaMemcpyDeviceToHost), "cudaMemcpy");
+        if (word != 0) cuda_check(cudaMemset(l->status_word.ptr, 0, sizeof(word)), "cudaMemset");
+        *out = static_cast<int32_t>(word);
     });
 }
 

@@ -4,7 +4,7 @@
 //
 // linear_step_kernel, the recurrent form: a CTA takes 32 columns of one head's state of one request into registers, goes through
 // the request's tokens and writes the columns back: bound by the state's bytes, read and written once for the whole run.  A
-// decay close to one that is rounded to f32 would be off by 2^-25 a token, and all in the same direction; it is held as two f32
+// decay close to one that is rounded to f32 would be off by up to 2^-25 a token, and all in the same direction; it is held as two f32
 // parts instead (lambda = hi + lo to 48 bits), one more multiply-add for each element and token.
 #include "device_common.cuh"
 #include "launch_util.hpp"
@@ -18,10 +18,6 @@ constexpr uint32_t kStepThreads = 128;
 constexpr uint32_t kStepColumns = 32;                       // of the state in one CTA: eight threads of four
 constexpr uint32_t kStepRowGroups = kStepThreads / 8;       // thread (group, four columns) holds rows group + 16 j
 constexpr uint32_t kStepTokens = 8;                         // tokens whose rows are in shared memory at once
-
-__device__ __forceinline__ float* state_of(const LinearParams& p, uint32_t slot, uint32_t head) {
-    return p.states + ((uint64_t(slot) * p.num_layers + p.layer) * p.num_v_heads + head) * p.key_dim * p.value_dim;
-}
 
 template <int kRows>  // of the state in one thread: key_dim <= 16 kRows
 __global__ __launch_bounds__(kStepThreads) void linear_step_kernel(const LinearParams p) {
@@ -38,7 +34,7 @@ __global__ __launch_bounds__(kStepThreads) void linear_step_kernel(const LinearP
         const LinearRequest rq = p.reqs[item / slices / p.num_v_heads];
         const uint32_t col = slice * kStepColumns + 4u * quad;
         const bool live = col < p.value_dim;  // value_dim is a multiple of eight
-        const float* from = state_of(p, rq.src, head);
+        const float* from = p.state_of(rq.src, head);
         float4 s[kRows];
 #pragma unroll
         for (int j = 0; j < kRows; ++j) {
@@ -46,7 +42,7 @@ __global__ __launch_bounds__(kStepThreads) void linear_step_kernel(const LinearP
             s[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (rq.fresh == 0 && live && row < p.key_dim) s[j] = *reinterpret_cast<const float4*>(from + uint64_t(row) * p.value_dim + col);
         }
-        const float hi = p.decays[head * kLinearDecays], lo = p.decays[head * kLinearDecays + 1];
+        const float hi = p.decays[head * kLinearDecays + 1], lo = p.decays[head * kLinearDecays + kLinearStepLow];
         for (uint32_t t0 = 0; t0 < rq.q_len; t0 += kStepTokens) {
             const uint32_t tokens = min(kStepTokens, rq.q_len - t0);
             __syncthreads();
@@ -97,7 +93,7 @@ __global__ __launch_bounds__(kStepThreads) void linear_step_kernel(const LinearP
                                      p.dtype, o * p.scale);
             }
         }
-        float* to = state_of(p, rq.dst, head);
+        float* to = p.state_of(rq.dst, head);
 #pragma unroll
         for (int j = 0; j < kRows; ++j) {
             const uint32_t row = group + kStepRowGroups * j;
