@@ -13,7 +13,9 @@ struct psi_linear {
     DeviceBuffer decays;       // [layers][Hv][kLinearDecays]
     DeviceBuffer status_word;  // u32 written by bounded device-side waits
     bool chunked = false;      // long runs take the chunked form
-    uint32_t num_steps = 0, num_runs = 0;  // of the prepared batch
+    DeviceBuffer carries;      // [max_carries][Hv][Dk][Dv]: states between the pieces of a request
+    uint32_t max_carries = 0;
+    uint32_t num_steps = 0, num_runs = 0, num_carries = 0, num_scans = 0, num_tokens = 0;  // of the prepared batch
     bool prepared = false;
     std::vector<uint32_t> reads, writes;  // by slot: readers of it in the batch at hand, and whether one writes it
 };
@@ -22,6 +24,47 @@ namespace {
 
 // Runs of more tokens take the chunked form.
 constexpr uint32_t kStepTokens = 16;
+
+// Into how many chunks the pieces of a batch's long runs are cut (0: nothing is cut).  The chunked form takes one CTA per run and head
+// through its chunks in turn, so that few heads leave SMs idle; pieces side by side cost a pass for the states between them.  In units
+// of a chunk's time (2.0 us at 128 x 128, the state pass's 0.5 of it): a launch takes the longest CTA's chunks, the CTAs going round
+// their items, and the scan with its two launches three.
+uint32_t piece_chunks(const std::vector<uint32_t>& run_tokens, uint32_t heads, uint32_t sms, uint32_t max_carries) {
+    uint32_t longest = 0;
+    const auto chunks_of = [](uint32_t tokens) { return (tokens + kLinearChunk - 1) / kLinearChunk; };
+    for (uint32_t tokens : run_tokens) longest = std::max(longest, chunks_of(tokens));
+    const auto cost = [&](uint32_t length) {  // pieces of `length` chunks
+        uint64_t items = 0, chunks = 0, carried = 0, carries = 0;
+        for (uint32_t tokens : run_tokens) {
+            const uint64_t c = chunks_of(tokens), pieces = (c + length - 1) / length;
+            items += pieces * heads;
+            chunks += c * heads;
+            if (pieces > 1) {
+                carried += (pieces - 1) * heads;
+                carries += pieces;
+            }
+        }
+        if (carries > max_carries) return 1e30;
+        const auto launch = [&](uint64_t n, uint64_t work) {
+            const double rounds = double((n + sms - 1) / sms);
+            return std::max(std::min(rounds * length, double(work)), double(work) / sms + 0.5 * length) + rounds;
+        };
+        const double full = launch(items, chunks);
+        return carried == 0 ? full : full + 0.5 * launch(carried, carried * length) + 3.0;
+    };
+    uint32_t best = 0;
+    double least = cost(longest);
+    for (uint32_t pieces = 2; pieces <= 32; ++pieces) {
+        const uint32_t length = (longest + pieces - 1) / pieces;
+        if (length < 2) break;
+        const double c = cost(length);
+        if (c < 0.95 * least) {
+            least = c;
+            best = length;
+        }
+    }
+    return best;
+}
 
 // What the kernels know of a head's decay (kLinearDecays).
 void fill_decay(float* out, float log_decay) {
@@ -62,10 +105,14 @@ int32_t psi_linear_create(psi_ctx* ctx, const psi_linear_config* config, psi_lin
         const uint64_t decays = uint64_t(c.num_layers) * c.num_v_heads;
         std::vector<float> none(decays * kLinearDecays);
         for (uint64_t i = 0; i < decays; ++i) fill_decay(none.data() + i * kLinearDecays, 0.0f);
+        // pieces for four rounds of CTAs
+        l->max_carries = std::max<uint32_t>(2, 4 * static_cast<uint32_t>(ctx->sm_count) / c.num_v_heads);
         l->chunked = linear_chunk_supported(c.dtype, c.key_dim, c.value_dim) && c.max_tokens > kStepTokens;
         try {
             l->block.ensure(ctx, block_capacity(l.get()) * sizeof(uint32_t), true);
             l->status_word.ensure(ctx, sizeof(uint32_t), true);
+            if (l->chunked && c.max_tokens > 2 * kLinearChunk)
+                l->carries.ensure(ctx, uint64_t(l->max_carries) * c.num_v_heads * c.key_dim * c.value_dim * sizeof(float), false);
             l->decays.ensure(ctx, none.size() * sizeof(float), false);
             cuda_check(cudaMemcpyAsync(l->decays.ptr, none.data(), none.size() * sizeof(float), cudaMemcpyHostToDevice, ctx->stream),
                        "cudaMemcpyAsync");  // pageable source: staged before the call returns
@@ -75,6 +122,7 @@ int32_t psi_linear_create(psi_ctx* ctx, const psi_linear_config* config, psi_lin
             l->block.release();
             l->decays.release();
             l->status_word.release();
+            l->carries.release();
             if (l->staging != nullptr) (void)cudaFreeHost(l->staging);
             throw;
         }
@@ -90,6 +138,7 @@ int32_t psi_linear_destroy(psi_linear* l) {
         l->block.release();
         l->decays.release();
         l->status_word.release();
+        l->carries.release();
         if (l->staging != nullptr) (void)cudaFreeHost(l->staging);
         if (l->upload_done != nullptr) (void)cudaEventDestroy(l->upload_done);
     });
@@ -159,17 +208,46 @@ int32_t psi_linear_prepare(psi_linear* l, const uint32_t* req_slots, const uint3
                 reqs[n++] = LinearRequest{req_slots[r], outs[r], token_indices[r] == 0 ? 1u : 0u, q_len, cu_tokens[r], {0, 0, 0}};
         }
         l->num_steps = n;
-        auto* runs = reinterpret_cast<LinearRun*>(reqs + n);
-        uint32_t num_runs = 0;
+        // the long runs in pieces: those that another one follows first, then the ends
+        std::vector<uint32_t> long_runs, run_tokens;
         for (uint32_t r = 0; r < num_reqs && l->chunked; ++r) {
-            const uint32_t q_len = cu_tokens[r + 1] - cu_tokens[r];
-            if (q_len > kStepTokens)
-                runs[num_runs++] = LinearRun{req_slots[r], outs[r], token_indices[r] == 0 ? 1u : 0u, 1, cu_tokens[r], q_len, kLinearNoCarry, kLinearNoCarry};
+            if (cu_tokens[r + 1] - cu_tokens[r] <= kStepTokens) continue;
+            long_runs.push_back(r);
+            run_tokens.push_back(cu_tokens[r + 1] - cu_tokens[r]);
         }
+        const uint32_t chunks = l->carries.ptr == nullptr || long_runs.empty()
+                                    ? 0
+                                    : piece_chunks(run_tokens, l->cfg.num_v_heads, static_cast<uint32_t>(ctx->sm_count), l->max_carries);
+        const uint32_t piece = chunks * kLinearChunk;  // tokens
+        auto* runs = reinterpret_cast<LinearRun*>(reqs + n);
+        std::vector<LinearRun> ends;
+        std::vector<LinearScan> scans;
+        uint32_t num_runs = 0, carry = 0;
+        for (uint32_t i = 0; i < long_runs.size(); ++i) {
+            const uint32_t r = long_runs[i], begin = cu_tokens[r], tokens = run_tokens[i], fresh = token_indices[r] == 0 ? 1u : 0u;
+            if (piece == 0 || tokens <= piece) {
+                ends.push_back(LinearRun{req_slots[r], outs[r], fresh, 1, begin, tokens, kLinearNoCarry, kLinearNoCarry});
+                continue;
+            }
+            const uint32_t pieces = (tokens + piece - 1) / piece;
+            scans.push_back(LinearScan{req_slots[r], fresh, carry, pieces, chunks, {0, 0, 0}});
+            for (uint32_t x = 0; x + 1 < pieces; ++x)
+                runs[num_runs++] = LinearRun{req_slots[r], outs[r], 0, 0, begin + x * piece, piece, carry + x, carry + x + 1};
+            ends.push_back(LinearRun{req_slots[r], outs[r], 0, 1, begin + (pieces - 1) * piece, tokens - (pieces - 1) * piece, carry + pieces - 1, kLinearNoCarry});
+            carry += pieces;
+        }
+        l->num_carries = num_runs;
+        std::stable_sort(ends.begin(), ends.end(), [](const LinearRun& a, const LinearRun& b) { return a.tokens > b.tokens; });
+        for (const LinearRun& run : ends) runs[num_runs++] = run;
+        std::memcpy(runs + num_runs, scans.data(), scans.size() * sizeof(LinearScan));
         l->num_runs = num_runs;
+        l->num_scans = static_cast<uint32_t>(scans.size());
+        l->num_tokens = cu_tokens[num_reqs];
         l->staging[kLinearNumSteps] = n;
         l->staging[kLinearNumRuns] = num_runs;
-        cuda_check(cudaMemcpyAsync(l->block.ptr, l->staging, (kLinearScalarCount + (n + num_runs) * kLinearRequestWords) * sizeof(uint32_t),
+        l->staging[kLinearNumCarries] = l->num_carries;
+        l->staging[kLinearNumScans] = l->num_scans;
+        cuda_check(cudaMemcpyAsync(l->block.ptr, l->staging, (kLinearScalarCount + uint64_t(n + num_runs + l->num_scans) * kLinearRequestWords) * sizeof(uint32_t),
                                    cudaMemcpyHostToDevice, ctx->stream),
                    "cudaMemcpyAsync");
         cuda_check(cudaEventRecord(l->upload_done, ctx->stream), "cudaEventRecord");
@@ -195,6 +273,7 @@ int32_t psi_linear_attend(psi_linear* l, uint32_t layer, float* states, const vo
         p.reqs = reinterpret_cast<const LinearRequest*>(p.scalars + kLinearScalarCount);
         p.decays = static_cast<const float*>(l->decays.ptr) + uint64_t(layer) * l->cfg.num_v_heads * kLinearDecays;
         p.states = states;
+        p.carries = static_cast<float*>(l->carries.ptr);
         p.q = q;
         p.k = k;
         p.v = v;
@@ -207,6 +286,7 @@ int32_t psi_linear_attend(psi_linear* l, uint32_t layer, float* states, const vo
         p.value_dim = l->cfg.value_dim;
         p.dtype = l->cfg.dtype;
         p.scale = l->cfg.scale;
+        p.num_tokens = ctx->capturing ? l->cfg.max_tokens : l->num_tokens;
         p.aligned = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0 ? 1u : 0u;
         const uint64_t wave = static_cast<uint64_t>(ctx->sm_count) * 16;
         const uint64_t per_request = uint64_t(l->cfg.num_v_heads) * linear_step_slices(l->cfg.value_dim);
@@ -217,11 +297,18 @@ int32_t psi_linear_attend(psi_linear* l, uint32_t layer, float* states, const vo
             cuda_check(launch_linear_step(p, static_cast<uint32_t>(std::min(items, wave)), ctx->stream), "linear attention launch");
         }
         const uint64_t sms = static_cast<uint64_t>(ctx->sm_count);
-        const uint64_t run_items = !l->chunked ? 0 : ctx->capturing ? sms : uint64_t(l->num_runs) * l->cfg.num_v_heads;
-        if (run_items > 0) {
+        const bool fixed = ctx->capturing;
+        const auto launch_runs = [&](bool state_only, uint64_t runs) {
+            const uint64_t ctas = fixed ? sms : std::min(sms, runs * l->cfg.num_v_heads);
             LaunchScope scope(ctx, PSI_KERNEL_CLASS_LINEAR);
-            cuda_check(launch_linear_chunk(p, false, static_cast<uint32_t>(std::min(run_items, sms)), ctx->stream), "linear attention (chunk) launch");
+            cuda_check(launch_linear_chunk(p, state_only, static_cast<uint32_t>(ctas), ctx->stream), "linear attention (chunk) launch");
+        };
+        if (l->carries.ptr != nullptr && (fixed || l->num_scans > 0)) {
+            launch_runs(true, l->num_carries);
+            LaunchScope scope(ctx, PSI_KERNEL_CLASS_LINEAR);
+            cuda_check(launch_linear_scan(p, ctx->stream), "linear attention (scan) launch");
         }
+        if (l->chunked && (fixed || l->num_runs > 0)) launch_runs(false, l->num_runs);
     });
 }
 

@@ -102,7 +102,44 @@ __global__ __launch_bounds__(kStepThreads) void linear_step_kernel(const LinearP
     }
 }
 
+// States before the pieces of a request, from the gains of the pieces: S of piece s + 1 = lambda^(tokens of piece s) S of piece s + its gain.
+// Bound by the carries' bytes, read and written once.
+__global__ __launch_bounds__(256) void linear_scan_kernel(const LinearParams p) {
+    await_previous_kernel();
+    const uint32_t count = p.scalars[kLinearNumScans], head = blockIdx.y;
+    const uint32_t elements = p.key_dim * p.value_dim / 4;
+    const uint32_t at = blockIdx.x * blockDim.x + threadIdx.x;
+    if (at >= elements) return;
+    const float* decay = p.decays + uint64_t(head) * kLinearDecays;
+    const double chunk = double(decay[kLinearChunk]) + double(decay[kLinearChunkLow]);
+    for (uint32_t i = 0; i < count; ++i) {
+        const LinearScan scan = p.scans()[i];
+        double power = 1.0, square = chunk;
+        for (uint32_t n = scan.piece_chunks; n != 0; n >>= 1, square *= square)
+            if (n & 1u) power *= square;
+        const float hi = float(power), lo = float(power - double(hi));
+        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (scan.fresh == 0) s = reinterpret_cast<const float4*>(p.state_of(scan.src, head))[at];
+        for (uint32_t piece = 0; piece < scan.pieces; ++piece) {
+            float4* carry = reinterpret_cast<float4*>(p.carry_of(scan.carry + piece, head)) + at;
+            if (piece > 0) {
+                const float4 gain = *carry;
+                s.x = fmaf(hi, s.x, fmaf(lo, s.x, gain.x));
+                s.y = fmaf(hi, s.y, fmaf(lo, s.y, gain.y));
+                s.z = fmaf(hi, s.z, fmaf(lo, s.z, gain.z));
+                s.w = fmaf(hi, s.w, fmaf(lo, s.w, gain.w));
+            }
+            *carry = s;
+        }
+    }
+}
+
 }  // namespace
+
+cudaError_t launch_linear_scan(const LinearParams& p, cudaStream_t stream) {
+    const uint32_t elements = p.key_dim * p.value_dim / 4;
+    return launch_overlapped(linear_scan_kernel, dim3((elements + 255) / 256, p.num_v_heads), dim3(256), 0, stream, p);
+}
 
 uint32_t linear_step_slices(uint32_t value_dim) { return (value_dim + kStepColumns - 1) / kStepColumns; }
 

@@ -21,6 +21,10 @@ bool make_kv_map(const AttendParams& p, uint32_t box_rows, CUtensorMap* map);
 // `box_rows / 8` consecutive groups, [group][K, V][element block]; its last coordinate is page * groups of a page + K group.
 bool make_kv_pair_map(const AttendParams& p, uint32_t box_rows, CUtensorMap* map);
 
+// Rows of `heads` heads of `dim` elements, [tokens][heads][dim], as [head][token][dim]: a box is `box_rows` tokens x 64 elements of
+// one head in the 128-byte swizzle, zeros beyond the head's elements and the tokens.
+bool make_rows_map(const void* base, uint32_t dtype, uint32_t dim, uint32_t heads, uint32_t tokens, uint32_t box_rows, CUtensorMap* map);
+
 __device__ __forceinline__ uint32_t smem_u32(const void* ptr) { return static_cast<uint32_t>(__cvta_generic_to_shared(ptr)); }
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }

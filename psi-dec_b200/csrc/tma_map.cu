@@ -57,5 +57,15 @@ bool make_kv_pair_map(const AttendParams& p, uint32_t box_rows, CUtensorMap* map
                       {64, 8, p.geo.head_dim / 64, 2, box_rows / 8}, map);
 }
 
+bool make_rows_map(const void* base, uint32_t dtype, uint32_t dim, uint32_t heads, uint32_t tokens, uint32_t box_rows, CUtensorMap* map) {
+    const EncodeTiled encode = encode_tiled();
+    if (encode == nullptr || reinterpret_cast<uintptr_t>(base) % 16 != 0 || dim % 8 != 0 || tokens == 0) return false;
+    const cuuint64_t dims[3] = {dim, tokens, heads}, strides[2] = {uint64_t(heads) * dim * 2, dim * 2ull};
+    const cuuint32_t box[3] = {64, box_rows, 1}, elem_strides[3] = {1, 1, 1};
+    const CUtensorMapDataType type = dtype == PSI_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return encode(map, type, 3, const_cast<void*>(base), dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 
 }  // namespace psi
