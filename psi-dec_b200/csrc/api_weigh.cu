@@ -225,7 +225,7 @@ int32_t psi_gqa_evict(psi_gqa* g, psi_pages* pages, psi_table* table, uint32_t l
         p.kept_stride = kept_stride;
         p.recent = recent;
         p.unit_bytes = copy_unit(p.geo);
-        const uint32_t wave = static_cast<uint32_t>(ctx->sm_count) * 4;
+        const uint32_t sms = static_cast<uint32_t>(ctx->sm_count);
         for (uint32_t first = 0; first < num_reqs; first += kEvictBatch) {
             p.num_reqs = std::min(kEvictBatch, num_reqs - first);
             p.kept = kept + uint64_t(first) * g->cfg.num_kv_heads * kept_stride;
@@ -239,13 +239,13 @@ int32_t psi_gqa_evict(psi_gqa* g, psi_pages* pages, psi_table* table, uint32_t l
             }
             {
                 LaunchScope scope(ctx, PSI_KERNEL_CLASS_EVICT);
-                cuda_check(launch_evict_select(p, ctx->stream), "eviction selection launch");
+                cuda_check(launch_evict_select(p, sms, ctx->stream), "eviction selection launch");
             }
             for (uint32_t way = 0; way < 2; ++way) {
                 if (!(way == 0 ? apart : in_place)) continue;
                 p.in_place = way;
                 LaunchScope scope(ctx, PSI_KERNEL_CLASS_EVICT);
-                cuda_check(launch_evict_move(p, wave, ctx->stream), "eviction move launch");
+                cuda_check(launch_evict_move(p, sms, ctx->stream), "eviction move launch");
             }
         }
     });

@@ -29,8 +29,8 @@ struct EvictParams {
     EvictRequest reqs[kEvictBatch];
 };
 
-cudaError_t launch_evict_select(const EvictParams& p, cudaStream_t stream);
-// Requests that keep their slot and requests that move to another one are two launches; `ctas` bounds the second.
-cudaError_t launch_evict_move(const EvictParams& p, uint32_t ctas, cudaStream_t stream);
+cudaError_t launch_evict_select(const EvictParams& p, uint32_t sms, cudaStream_t stream);
+// Requests that keep their slot and requests that move to another one are two launches.
+cudaError_t launch_evict_move(const EvictParams& p, uint32_t sms, cudaStream_t stream);
 
 }  // namespace psi
