@@ -71,7 +71,7 @@ int32_t psi_gqa_destroy(psi_gqa* g) {
         g->sync_words.release();
         g->xchg_local.release();
         g->norm_rope.release();
-        g->weigh.lse.release();
+        g->weigh.norms.release();
         g->weigh.partials.release();
         g->weigh.counters.release();
         g->weigh.scores.release();

@@ -201,7 +201,7 @@ struct psi_weigh_plan {
     bool captured = false;               // a captured launch sequence holds key-weight launches
     std::vector<uint32_t> seen;          // by slot: the epoch that last named it
     uint32_t epoch = 0;
-    psi::DeviceBuffer lse, partials, counters, scores;
+    psi::DeviceBuffer norms, partials, counters, scores;
 };
 
 struct psi_gqa {

@@ -48,7 +48,7 @@ void plan_weigh(psi_gqa* g, const uint32_t* req_slots, const uint32_t* token_ind
                 const uint64_t units = (rows + block - 1) / block * heads;
                 w.long_units += units;
                 cu0 += units * weigh_pieces(keys);
-                cu1 += (uint64_t(keys) + kWeighBlock - 1) / kWeighBlock * heads;
+                cu1 += weigh_sum_items(keys, tensor) * heads;
             }
         }
         WeighRequest end{};
@@ -115,7 +115,7 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
         const uint32_t block = tensor ? kWeighBlock : kWeighAnyRows;
         const bool can_short = tensor, can_long = !tensor || uint64_t(g->cfg.max_tokens) * group > kWeighShortRows;
         // one wave of the short-run kernel's workers
-        const uint64_t short_wave = sms * (g->cfg.head_dim <= 128 ? 2 : 1);
+        const uint64_t short_wave = sms * 2;
         const uint64_t short_ctas = fixed ? (can_short ? short_wave : 0) : std::min<uint64_t>(short_wave, (w.tiles + 7) / 8);
         uint64_t short_units = uint64_t(w.num_short) * heads, long_units = w.long_units, stats_items = w.stats_items;
         if (fixed) {
@@ -128,13 +128,13 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
         const uint64_t partial_bytes = (short_slots + long_slots) * sizeof(float2);
         const uint64_t counter_words = short_units + long_units;
         if (ctx->capturing) {
-            require(w.lse.ptr != nullptr && partial_bytes <= w.partials.bytes && counter_words * sizeof(uint32_t) <= w.counters.bytes,
+            require(w.norms.ptr != nullptr && partial_bytes <= w.partials.bytes && counter_words * sizeof(uint32_t) <= w.counters.bytes,
                     "call psi_gqa_weigh_keys once after the replay reservation and before the capture: it allocates its scratch then");
         } else {
             require(!fixed || partial_bytes <= (2ull << 30),
                     "the replay reservation needs more than 2 GiB of key-weight scratch for this max_tokens: create the component with "
                     "the largest batch the replayed steps carry");
-            w.lse.ensure(ctx, uint64_t(g->cfg.max_tokens) * g->cfg.num_q_heads * sizeof(float), false);
+            w.norms.ensure(ctx, uint64_t(g->cfg.max_tokens) * g->cfg.num_q_heads * sizeof(float2), false);
             w.partials.ensure(ctx, partial_bytes > w.partials.bytes ? std::max<uint64_t>(partial_bytes * 3 / 2, 1 << 16) : partial_bytes, false);
             if (counter_words * sizeof(uint32_t) > w.counters.bytes) {
                 w.counters.release_after(ctx);  // counters restart from zero at their new size
@@ -146,7 +146,7 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
         p.stride = weights_stride;
         p.reqs = reinterpret_cast<const WeighRequest*>(block_words(g, g->off_weigh));
         p.scalars = block_words(g, 0);
-        p.lse = static_cast<float*>(w.lse.ptr);
+        p.norms = static_cast<float2*>(w.norms.ptr);
         p.partials = static_cast<float2*>(w.partials.ptr);
         p.long_partials_at = short_slots;
         p.counters = static_cast<uint32_t*>(w.counters.ptr);
@@ -155,7 +155,7 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
         p.num_q_heads = g->cfg.num_q_heads;
         p.dtype = g->cfg.dtype;
         p.scale_log2 = g->cfg.scale * 1.4426950408889634f;
-        p.score_rows = w.short_rows <= 8 ? 8 : 16;
+        p.score_rows = w.short_rows;
         bool keep_scores = false;
         if (short_ctas > 0 && !fixed) {
             // The scores of short runs stay in scratch between the passes; beyond 2 GiB, or where the device has no room left,
@@ -173,8 +173,9 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
         }
         if (ctx->capturing) w.captured = true;
         if (short_ctas > 0) run_pass(g, p, keep_scores ? WeighPass::kShortStatsScores : WeighPass::kShortStats, short_ctas);
-        const uint64_t stats_ctas = fixed ? (can_long ? sms * 8 : 0) : std::min<uint64_t>(sms * 8, w.stats_items);
-        const uint64_t sum_ctas = fixed ? stats_ctas : std::min<uint64_t>(sms * 8, w.sum_items);
+        const uint64_t long_wave = sms * (tensor ? 2 : 8);
+        const uint64_t stats_ctas = fixed ? (can_long ? long_wave : 0) : std::min<uint64_t>(long_wave, w.stats_items);
+        const uint64_t sum_ctas = fixed ? stats_ctas : std::min<uint64_t>(long_wave, w.sum_items);
         if (stats_ctas > 0) run_pass(g, p, WeighPass::kLongStats, stats_ctas);
         if (short_ctas > 0) {
             const uint64_t ctas = keep_scores ? std::min<uint64_t>(sms * 8, (w.tiles + 7) / 8) : short_ctas;

@@ -160,7 +160,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return v;
 }
 
-// The same of magnitudes, and no number where one of them is none.
+// The same, and no number where one of them is none; and of magnitudes.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float v;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+    return v;
+}
 __device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
     float v;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));

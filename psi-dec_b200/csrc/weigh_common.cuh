@@ -1,0 +1,70 @@
+// What the key-weight kernels share: where requests, rows and keys lie, and the numbers of a row's softmax.
+#pragma once
+
+#include "mma_common.cuh"
+#include "weigh_keys.hpp"
+
+namespace psi {
+
+constexpr float kInf = INFINITY;
+
+__device__ __forceinline__ float exp2_approx(float x) {  // 2 ulp; results below the smallest normal number are 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The request whose work holds `index`: the last one whose prefix (`which` 0: cu0, 1: cu1) is at or below it.
+template <int kWhich>
+__device__ __forceinline__ uint32_t find_request(const WeighRequest* reqs, uint32_t count, uint32_t index) {
+    uint32_t lo = 0, hi = count;  // invariant: prefix[lo] <= index < prefix[hi]
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if ((kWhich == 0 ? reqs[mid].cu0 : reqs[mid].cu1) <= index) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// (maximum, sum) of a row's scores in the log2 domain; an empty one is (-inf, 0).
+struct Stat {
+    float m, l;
+    __device__ __forceinline__ void join(float m2, float l2) {
+        const float top = fmaxf(m, m2);
+        const float base = top == -kInf ? 0.0f : top;
+        l = l * exp2f(m - base) + l2 * exp2f(m2 - base);
+        m = top;
+    }
+    // What the second pass takes of the row: (maximum, 1 / sum), or (inf, 0) for a row that adds nothing.
+    __device__ __forceinline__ float2 norm() const {
+        return l > 0.0f && l < kInf && fabsf(m) < kInf ? make_float2(m, 1.0f / l) : make_float2(kInf, 0.0f);
+    }
+};
+
+// The weight of a key from its product with the query row.
+__device__ __forceinline__ float weight_of(float product, float scale_log2, float2 norm) {
+    return norm.y > 0.0f ? exp2_approx(fmaf(product, scale_log2, -norm.x)) * norm.y : 0.0f;
+}
+
+// Query row r of a request and KV head as (flat token, head) row of q.
+__device__ __forceinline__ uint64_t query_row(const WeighParams& p, const WeighRequest& rq, uint32_t head, uint32_t r) {
+    return uint64_t(rq.flat_begin + r / p.group) * p.num_q_heads + head * p.group + r % p.group;
+}
+
+// Keys that row r sees.
+__device__ __forceinline__ uint32_t row_limit(const WeighParams& p, const WeighRequest& rq, uint32_t r) {
+    return rq.first_pos + r / p.group + 1;
+}
+
+__device__ __forceinline__ const uint4* key_row(const WeighParams& p, const PageBounds& bounds, const uint32_t* row_ids,
+                                                uint32_t head, uint32_t key, uint32_t& bad) {
+    const uint32_t page = bounds.read(row_ids, key / p.geo.tokens_per_page, bad);
+    const uint64_t at = kv_row_offset(p.geo, page, head, key % p.geo.tokens_per_page);
+    return reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.geo.pages) + at);
+}
+
+__device__ __forceinline__ float* weight_row(const WeighParams& p, const WeighRequest& rq, uint32_t head) {
+    return p.weights + (uint64_t(rq.slot) * p.geo.num_kv_heads + head) * p.stride;
+}
+
+}  // namespace psi

@@ -4,74 +4,31 @@
 //                                exp(scale q_r . k_j - M_r) / L_r        for j <= token_index + i
 //
 // with M_r and L_r the maximum and the exponential sum of row r's scores.  A row without a finite maximum or sum adds nothing.
-// Two passes, since no weight is known before its row's sum is: the first finds log2-domain normalisers, the second adds up
+// Two passes, since no weight is known before its row's sum is: the first finds M and 1 / L, the second adds up
 // columns.  Both keep f32 scores; every key's sum is worked out by one thread group in one order, so results repeat bit for bit.
+// M and 1 / L stay apart: their logarithmic sum is a number of twenty or so, whose rounding alone would be the largest error.
 //
 //   weigh_short_kernel   runs of up to 16 rows (decode, drafts): bound by the K bytes.  One warp is one worker with an equal
 //                        share of the batch's 32-key tiles.  Products do not depend on the order of the columns of q and k, so
 //                        a lane takes 16 consecutive bytes of a key row as the operands of two m16n8k16 steps, and the
-//                        same bytes of the query rows: K goes from HBM to registers with no shared memory and no barrier, for any
+//                        same bytes of the query rows (from shared memory): K goes from HBM to registers with no barrier, for any
 //                        page size.  The first pass leaves its scores in scratch, 4 bytes a row and key against 2 head_dim
 //                        bytes a key, so that K is read once; where there is no scratch (captured launches, very
 //                        large batches) the second pass reads K again.
-//   weigh_stats_kernel,  longer runs: 64 rows (first pass) or 64 keys (second pass) stay in registers as the A operand, blocks
-//   weigh_sum_kernel     of 64 keys or rows pass through shared memory as the B operand.  In the second pass the keys are the
-//                        rows of the product, so a column sum stays inside a thread until its end.
+//   weigh_umma_kernel    longer runs, on tcgen05 (weigh_umma.cu).
 //   weigh_*_any_kernel   f32 and head dims that are no multiple of eight: the same two passes in f32 on the CUDA cores.
 #include "mma_common.cuh"
 #include "launch_util.hpp"
-#include "weigh_keys.hpp"
+#include "weigh_common.cuh"
 
 namespace psi {
 
 namespace {
 
-constexpr float kInf = INFINITY;
-
 __device__ __forceinline__ uint4 ld_stream(const uint4* p) {
     uint4 v;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
-}
-
-// The request whose work holds `index`: the last one whose prefix (`which` 0: cu0, 1: cu1) is at or below it.
-template <int kWhich>
-__device__ __forceinline__ uint32_t find_request(const WeighRequest* reqs, uint32_t count, uint32_t index) {
-    uint32_t lo = 0, hi = count;  // invariant: prefix[lo] <= index < prefix[hi]
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if ((kWhich == 0 ? reqs[mid].cu0 : reqs[mid].cu1) <= index) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
-
-// (maximum, sum) of a row's scores in the log2 domain; an empty one is (-inf, 0).
-struct Stat {
-    float m, l;
-    __device__ __forceinline__ void join(float m2, float l2) {
-        const float top = fmaxf(m, m2);
-        const float base = top == -kInf ? 0.0f : top;
-        l = l * exp2f(m - base) + l2 * exp2f(m2 - base);
-        m = top;
-    }
-    // The normaliser subtracted from the row's scores: +inf tells that the row adds nothing.
-    __device__ __forceinline__ float lse() const {
-        const float v = m + log2f(l);
-        return l > 0.0f && fabsf(v) < kInf ? v : kInf;
-    }
-};
-
-__device__ __forceinline__ float weight_of(float score, float lse) { return lse < kInf ? exp2f(score - lse) : 0.0f; }
-
-// Query row r of a request and KV head as (flat token, head) row of q.
-__device__ __forceinline__ uint64_t query_row(const WeighParams& p, const WeighRequest& rq, uint32_t head, uint32_t r) {
-    return uint64_t(rq.flat_begin + r / p.group) * p.num_q_heads + head * p.group + r % p.group;
-}
-
-// Keys that row r sees.
-__device__ __forceinline__ uint32_t row_limit(const WeighParams& p, const WeighRequest& rq, uint32_t r) {
-    return rq.first_pos + r / p.group + 1;
 }
 
 // 16-byte chunks of a 16-bit row that a lane holds: chunk (lane & 3) + 4 i for i < NC, zeros beyond the row.
@@ -84,17 +41,7 @@ __device__ __forceinline__ void load_row(uint4 (&x)[NC], const uint4* row, uint3
     }
 }
 
-// A operand: rows quad_row and quad_row + 8.
-template <int NC>
-struct RowPair {
-    uint4 lo[NC], hi[NC];
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int i = 0; i < NC; ++i) lo[i] = hi[i] = make_uint4(0, 0, 0, 0);
-    }
-};
-
-// d += A B for the two steps that one 16-byte chunk of every row makes.
+// d += A B for the two steps that one 16-byte chunk of every row makes; lo, hi: rows quad_row and quad_row + 8 of A.
 template <typename T>
 __device__ __forceinline__ void chunk_mma(float (&d)[4], const uint4& lo, const uint4& hi, const uint4& b) {
     const uint32_t a0[4] = {lo.x, hi.x, lo.y, hi.y}, a1[4] = {lo.z, hi.z, lo.w, hi.w};
@@ -102,21 +49,18 @@ __device__ __forceinline__ void chunk_mma(float (&d)[4], const uint4& lo, const 
     Mma<T>::run(d, a1, b.z, b.w);
 }
 
-__device__ __forceinline__ const uint4* key_row(const WeighParams& p, const PageBounds& bounds, const uint32_t* row_ids,
-                                                uint32_t head, uint32_t key, uint32_t& bad) {
-    const uint32_t page = bounds.read(row_ids, key / p.geo.tokens_per_page, bad);
-    const uint64_t at = kv_row_offset(p.geo, page, head, key % p.geo.tokens_per_page);
-    return reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.geo.pages) + at);
-}
-
-__device__ __forceinline__ float* weight_row(const WeighParams& p, const WeighRequest& rq, uint32_t head) {
-    return p.weights + (uint64_t(rq.slot) * p.geo.num_kv_heads + head) * p.stride;
+// Byte offset of 16-byte chunk `chunk` of row `row` in a block of NC * 64-byte rows: the eight lanes of one phase of a 16-byte read
+// (two rows, four chunks) fall into distinct banks.
+template <int NC>
+__device__ __forceinline__ uint32_t block_offset(uint32_t row, uint32_t chunk) {
+    return row * (NC * 64u) + ((NC % 2 == 0 ? chunk ^ ((row & 1u) << 2) : chunk) << 4);
 }
 
 enum ShortMode { kStatsAndScores = 0, kStatsOnly = 1, kSumAgain = 2 };
 
 template <typename T, int NC, int kMode>
-__global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void weigh_short_kernel(const WeighParams p) {
+__global__ __launch_bounds__(256, 2) void weigh_short_kernel(const WeighParams p) {
+    extern __shared__ __align__(128) unsigned char smem[];
     await_previous_kernel();
     const uint32_t count = p.scalars[kScalarWeighShort];
     if (count == 0) return;
@@ -125,6 +69,7 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void weigh_short_kernel(const
     const uint32_t workers = min(gridDim.x * 8u, total);
     const uint32_t w = blockIdx.x * 8u + (threadIdx.x >> 5);
     if (w >= workers) return;
+    unsigned char* q_rows = smem + (threadIdx.x >> 5) * (16 * NC * 64);  // this warp's
     const uint32_t lane = threadIdx.x & 31u, quad_row = lane >> 2, quad_col = lane & 3u;
     const uint32_t begin = uint32_t(uint64_t(w) * total / workers), end = uint32_t(uint64_t(w + 1) * total / workers);
     const uint32_t chunks = p.geo.head_dim >> 3;
@@ -140,17 +85,28 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void weigh_short_kernel(const
         const uint32_t last = min(end, unit_end);
         const uint32_t rows = rq.q_len * p.group;
         const uint32_t* row_ids = table_row(p.geo, rq.slot);
-        RowPair<NC> q;
-        q.zero();
-        if (quad_row < rows) load_row<NC>(q.lo, reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + query_row(p, rq, head, quad_row) * p.geo.head_dim), quad_col, chunks);
-        if (quad_row + 8 < rows) load_row<NC>(q.hi, reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + query_row(p, rq, head, quad_row + 8) * p.geo.head_dim), quad_col, chunks);
+        // the unit's query rows, zeros behind them
+        __syncwarp();
+#pragma unroll
+        for (uint32_t half = 0; half < 2; ++half) {
+            const uint32_t row = quad_row + 8 * half;
+            uint4 x[NC];
+#pragma unroll
+            for (int i = 0; i < NC; ++i) x[i] = make_uint4(0, 0, 0, 0);
+            if (row < rows)
+                load_row<NC>(x, reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + query_row(p, rq, head, row) * p.geo.head_dim), quad_col, chunks);
+#pragma unroll
+            for (int i = 0; i < NC; ++i) *reinterpret_cast<uint4*>(q_rows + block_offset<NC>(row, quad_col + 4u * i)) = x[i];
+        }
+        __syncwarp();
+        const bool two_halves = rows > 8;
         const uint32_t limit0 = quad_row < rows ? row_limit(p, rq, quad_row) : 0u;
         const uint32_t limit1 = quad_row + 8 < rows ? row_limit(p, rq, quad_row + 8) : 0u;
         Stat s0{-kInf, 0.0f}, s1{-kInf, 0.0f};
-        float lse0 = kInf, lse1 = kInf;
+        float2 norm0 = make_float2(kInf, 0.0f), norm1 = norm0;
         if (kMode == kSumAgain) {
-            if (quad_row < rows) lse0 = p.lse[query_row(p, rq, head, quad_row)];
-            if (quad_row + 8 < rows) lse1 = p.lse[query_row(p, rq, head, quad_row + 8)];
+            if (quad_row < rows) norm0 = p.norms[query_row(p, rq, head, quad_row)];
+            if (quad_row + 8 < rows) norm1 = p.norms[query_row(p, rq, head, quad_row + 8)];
         }
         constexpr int kBatch = NC <= 4 ? 4 : 2;  // 8-key groups whose rows are in flight at once
         for (; tile < last; ++tile) {
@@ -163,26 +119,30 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void weigh_short_kernel(const
                     const uint32_t key = min(key0 + 8u * (half + t) + quad_row, rq.keys - 1u);
                     load_row<NC>(k[t], key_row(p, bounds, row_ids, head, key, bad), quad_col, chunks);
                 }
-                float s[kBatch][4];
+                float s[kBatch][4];  // products, -inf where a row does not see a key
 #pragma unroll
-                for (int t = 0; t < kBatch; ++t) {
-                    s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
+                for (int t = 0; t < kBatch; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < NC; ++i) chunk_mma<T>(s[t], q.lo[i], q.hi[i], k[t][i]);
+                for (int i = 0; i < NC; ++i) {
+                    const uint4 lo = *reinterpret_cast<const uint4*>(q_rows + block_offset<NC>(quad_row, quad_col + 4u * i));
+                    uint4 hi = make_uint4(0, 0, 0, 0);
+                    if (two_halves) hi = *reinterpret_cast<const uint4*>(q_rows + block_offset<NC>(quad_row + 8, quad_col + 4u * i));
+#pragma unroll
+                    for (int t = 0; t < kBatch; ++t) chunk_mma<T>(s[t], lo, hi, k[t][i]);
                 }
 #pragma unroll
                 for (int t = 0; t < kBatch; ++t) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const uint32_t key = key0 + 8u * (half + t) + 2u * quad_col + (e & 1);
-                        s[t][e] = key < (e < 2 ? limit0 : limit1) ? s[t][e] * p.scale_log2 : -kInf;
+                        s[t][e] = key < (e < 2 ? limit0 : limit1) ? s[t][e] : -kInf;
                     }
                 }
                 if (kMode == kSumAgain) {
 #pragma unroll
                     for (int t = 0; t < kBatch; ++t) {
-                        float a = weight_of(s[t][0], lse0) + weight_of(s[t][2], lse1);
-                        float b = weight_of(s[t][1], lse0) + weight_of(s[t][3], lse1);
+                        float a = weight_of(s[t][0], p.scale_log2, norm0) + weight_of(s[t][2], p.scale_log2, norm1);
+                        float b = weight_of(s[t][1], p.scale_log2, norm0) + weight_of(s[t][3], p.scale_log2, norm1);
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) {
                             a += __shfl_xor_sync(0xFFFFFFFFu, a, x);
@@ -195,28 +155,31 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void weigh_short_kernel(const
                     }
                 } else {
                     if (kMode == kStatsAndScores) {
+                        // [8-key group][row][8 keys], as many rows as the batch's longest run has
 #pragma unroll
                         for (int t = 0; t < kBatch; ++t) {
                             float* at = p.scores + (uint64_t(tile) * 4u + half + t) * 8u * p.score_rows + quad_row * 8u + 2u * quad_col;
-                            *reinterpret_cast<float2*>(at) = make_float2(s[t][0], s[t][1]);
-                            if (p.score_rows > 8) *reinterpret_cast<float2*>(at + 64) = make_float2(s[t][2], s[t][3]);
+                            if (quad_row < p.score_rows) *reinterpret_cast<float2*>(at) = make_float2(s[t][0], s[t][1]);
+                            if (quad_row + 8 < p.score_rows) *reinterpret_cast<float2*>(at + 64) = make_float2(s[t][2], s[t][3]);
                         }
                     }
-                    float m0 = s0.m, m1 = s1.m;
+                    float m0 = -kInf, m1 = -kInf;
 #pragma unroll
                     for (int t = 0; t < kBatch; ++t) {
                         m0 = fmaxf(m0, fmaxf(s[t][0], s[t][1]));
                         m1 = fmaxf(m1, fmaxf(s[t][2], s[t][3]));
                     }
+                    m0 = fmaxf(s0.m, m0 * p.scale_log2);
+                    m1 = fmaxf(s1.m, m1 * p.scale_log2);
                     const float base0 = m0 == -kInf ? 0.0f : m0, base1 = m1 == -kInf ? 0.0f : m1;
-                    s0.l *= exp2f(s0.m - base0);
-                    s1.l *= exp2f(s1.m - base1);
+                    s0.l *= exp2_approx(s0.m - base0);
+                    s1.l *= exp2_approx(s1.m - base1);
                     s0.m = m0;
                     s1.m = m1;
 #pragma unroll
                     for (int t = 0; t < kBatch; ++t) {
-                        s0.l += exp2f(s[t][0] - base0) + exp2f(s[t][1] - base0);
-                        s1.l += exp2f(s[t][2] - base1) + exp2f(s[t][3] - base1);
+                        s0.l += exp2_approx(fmaf(s[t][0], p.scale_log2, -base0)) + exp2_approx(fmaf(s[t][1], p.scale_log2, -base0));
+                        if (two_halves) s1.l += exp2_approx(fmaf(s[t][2], p.scale_log2, -base1)) + exp2_approx(fmaf(s[t][3], p.scale_log2, -base1));
                     }
                 }
             }
@@ -232,8 +195,8 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void weigh_short_kernel(const
         const uint32_t first_worker = uint32_t((uint64_t(unit_begin + 1) * workers - 1) / total);
         const uint32_t last_worker = uint32_t((uint64_t(unit_end) * workers - 1) / total);
         if (first_worker == last_worker) {
-            if (quad_col == 0 && quad_row < rows) p.lse[query_row(p, rq, head, quad_row)] = s0.lse();
-            if (quad_col == 0 && quad_row + 8 < rows) p.lse[query_row(p, rq, head, quad_row + 8)] = s1.lse();
+            if (quad_col == 0 && quad_row < rows) p.norms[query_row(p, rq, head, quad_row)] = s0.norm();
+            if (quad_col == 0 && quad_row + 8 < rows) p.norms[query_row(p, rq, head, quad_row + 8)] = s1.norm();
             continue;
         }
         // worker + unit grows from one segment of the batch to the next: a slot of its own for each
@@ -256,7 +219,7 @@ __global__ __launch_bounds__(256, NC <= 4 ? 2 : 1) void weigh_short_kernel(const
                 s.join(v.x, v.y);
             }
             s.join(__shfl_xor_sync(0xFFFFFFFFu, s.m, 16), __shfl_xor_sync(0xFFFFFFFFu, s.l, 16));
-            if (lane < rows) p.lse[query_row(p, rq, head, lane)] = s.lse();
+            if (lane < rows) p.norms[query_row(p, rq, head, lane)] = s.norm();
             if (lane == 0) p.counters[unit] = 0;
         }
     }
@@ -284,242 +247,15 @@ __global__ __launch_bounds__(256) void weigh_scores_kernel(const WeighParams p) 
         const uint32_t rows = rq.q_len * p.group;
         const float* s = p.scores + (uint64_t(tile) * 4u + (lane >> 3)) * 8u * p.score_rows + (lane & 7u);
         float sum = 0.0f;
-        for (uint32_t r = 0; r < rows; ++r) sum += weight_of(s[r * 8u], p.lse[query_row(p, rq, head, r)]);
+        #pragma unroll 4
+        for (uint32_t r = 0; r < rows; ++r) sum += weight_of(s[r * 8u], p.scale_log2, p.norms[query_row(p, rq, head, r)]);
         if (key < rq.keys) weight_row(p, rq, head)[key] += sum;
     }
 }
 
-// ---- runs of more than 16 rows -------------------------------------------------------------------------------------------
-
-constexpr uint32_t kBlock = kWeighBlock;  // rows or keys of one A block, and of one B block
-
-// Byte offset of 16-byte chunk `chunk` of row `row` in a B block of NC * 64-byte rows: the eight lanes of one phase of a
-// 16-byte read (two rows, four chunks) fall into distinct banks.
-template <int NC>
-__device__ __forceinline__ uint32_t block_offset(uint32_t row, uint32_t chunk) {
-    return row * (NC * 64u) + ((NC % 2 == 0 ? chunk ^ ((row & 1u) << 2) : chunk) << 4);
-}
-
-// The 64 x 64 product of a warp's 16 A rows and the B block in shared memory.
-template <typename T, int NC>
-__device__ __forceinline__ void block_product(float (&s)[8][4], const RowPair<NC>& a, const unsigned char* b, uint32_t quad_row,
-                                              uint32_t quad_col) {
-#pragma unroll
-    for (int t = 0; t < 8; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            const uint4 v = *reinterpret_cast<const uint4*>(b + block_offset<NC>(8u * t + quad_row, quad_col + 4u * i));
-            chunk_mma<T>(s[t], a.lo[i], a.hi[i], v);
-        }
-    }
-}
-
-template <int NC>
-__device__ __forceinline__ void copy_row(uint32_t smem, uint32_t row, const uint4* src, bool live, uint32_t chunks) {
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        const uint32_t c = (threadIdx.x & 3u) + 4u * i;
-        cp_async_16(smem + block_offset<NC>(row, c), src + (c < chunks ? c : 0u), live && c < chunks ? 16u : 0u);
-    }
-}
-
-// First pass: item = (request, KV head, 64 rows, piece of the keys).
-template <typename T, int NC>
-__global__ __launch_bounds__(128) void weigh_stats_kernel(const WeighParams p) {
-    extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ uint32_t last_arrival;
-    await_previous_kernel();
-    const uint32_t count = p.scalars[kScalarWeighLong];
-    if (count == 0) return;
-    const WeighRequest* reqs = p.long_reqs();
-    const uint32_t total = reqs[count].cu0;
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, quad_row = lane >> 2, quad_col = lane & 3u;
-    const uint32_t chunks = p.geo.head_dim >> 3;
-    const uint32_t smem_base = uint32_t(__cvta_generic_to_shared(smem));
-    const PageBounds bounds(p.geo);
-    uint32_t bad = 0;
-    for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
-        const uint32_t r_index = find_request<0>(reqs, count, item);
-        const WeighRequest rq = reqs[r_index];
-        const uint32_t pieces = weigh_pieces(rq.keys), rows = rq.q_len * p.group, blocks = (rows + kBlock - 1) / kBlock;
-        const uint32_t local = item - rq.cu0, piece = local % pieces, unit = local / pieces;
-        const uint32_t head = unit / blocks, row0 = (unit % blocks) * kBlock;
-        const uint32_t piece_keys = weigh_piece_keys(rq.keys, pieces);
-        const uint32_t seen = row_limit(p, rq, min(row0 + kBlock, rows) - 1);
-        const uint32_t k0 = piece * piece_keys, k1 = min(min(k0 + piece_keys, rq.keys), seen);
-        const uint32_t* row_ids = table_row(p.geo, rq.slot);
-        const uint32_t ra = row0 + warp * 16u + quad_row, rb = ra + 8u;
-        const uint32_t limit0 = ra < rows ? row_limit(p, rq, ra) : 0u, limit1 = rb < rows ? row_limit(p, rq, rb) : 0u;
-        Stat s0{-kInf, 0.0f}, s1{-kInf, 0.0f};
-        if (k0 < k1) {
-            RowPair<NC> q;
-            q.zero();
-            if (ra < rows) load_row<NC>(q.lo, reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + query_row(p, rq, head, ra) * p.geo.head_dim), quad_col, chunks);
-            if (rb < rows) load_row<NC>(q.hi, reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + query_row(p, rq, head, rb) * p.geo.head_dim), quad_col, chunks);
-            const auto fetch = [&](uint32_t key0, uint32_t stage) {
-#pragma unroll
-                for (uint32_t half = 0; half < 2; ++half) {
-                    const uint32_t row = (threadIdx.x >> 2) + 32u * half, key = key0 + row;
-                    copy_row<NC>(smem_base + stage * (kBlock * NC * 64u), row, key_row(p, bounds, row_ids, head, min(key, k1 - 1), bad), key < k1, chunks);
-                }
-                cp_async_commit();
-            };
-            fetch(k0, 0);
-            uint32_t stage = 0;
-            for (uint32_t key0 = k0; key0 < k1; key0 += kBlock, stage ^= 1u) {
-                if (key0 + kBlock < k1) {
-                    fetch(key0 + kBlock, stage ^ 1u);
-                    cp_async_wait<1>();
-                } else {
-                    cp_async_wait<0>();
-                }
-                __syncthreads();
-                float s[8][4];
-                block_product<T, NC>(s, q, smem + stage * (kBlock * NC * 64u), quad_row, quad_col);
-                float m0 = s0.m, m1 = s1.m;
-#pragma unroll
-                for (int t = 0; t < 8; ++t) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t key = key0 + 8u * t + 2u * quad_col + (e & 1);
-                        s[t][e] = key < min(k1, e < 2 ? limit0 : limit1) ? s[t][e] * p.scale_log2 : -kInf;
-                    }
-                    m0 = fmaxf(m0, fmaxf(s[t][0], s[t][1]));
-                    m1 = fmaxf(m1, fmaxf(s[t][2], s[t][3]));
-                }
-                const float base0 = m0 == -kInf ? 0.0f : m0, base1 = m1 == -kInf ? 0.0f : m1;
-                s0.l *= exp2f(s0.m - base0);
-                s1.l *= exp2f(s1.m - base1);
-                s0.m = m0;
-                s1.m = m1;
-#pragma unroll
-                for (int t = 0; t < 8; ++t) {
-                    s0.l += exp2f(s[t][0] - base0) + exp2f(s[t][1] - base0);
-                    s1.l += exp2f(s[t][2] - base1) + exp2f(s[t][3] - base1);
-                }
-                __syncthreads();
-            }
-#pragma unroll
-            for (int x = 1; x < 4; x <<= 1) {
-                s0.join(__shfl_xor_sync(0xFFFFFFFFu, s0.m, x), __shfl_xor_sync(0xFFFFFFFFu, s0.l, x));
-                s1.join(__shfl_xor_sync(0xFFFFFFFFu, s1.m, x), __shfl_xor_sync(0xFFFFFFFFu, s1.l, x));
-            }
-        }
-        if (pieces == 1) {
-            if (quad_col == 0 && ra < rows) p.lse[query_row(p, rq, head, ra)] = s0.lse();
-            if (quad_col == 0 && rb < rows) p.lse[query_row(p, rq, head, rb)] = s1.lse();
-            continue;
-        }
-        float2* slot = p.long_partials() + uint64_t(item) * kBlock;
-        if (quad_col == 0) {
-            slot[warp * 16u + quad_row] = make_float2(s0.m, s0.l);
-            slot[warp * 16u + quad_row + 8u] = make_float2(s1.m, s1.l);
-        }
-        __threadfence();
-        __syncthreads();
-        uint32_t* counter = p.long_counters() + rq.unit0 + unit;
-        if (threadIdx.x == 0) last_arrival = atomicAdd(counter, 1u) == pieces - 1 ? 1u : 0u;
-        __syncthreads();
-        if (last_arrival != 0) {
-            __threadfence();
-            const uint32_t row = row0 + threadIdx.x;
-            if (threadIdx.x < kBlock && row < rows) {
-                Stat s{-kInf, 0.0f};
-                for (uint32_t o = 0; o < pieces; ++o) {
-                    const float2 v = __ldcg(p.long_partials() + uint64_t(rq.cu0 + unit * pieces + o) * kBlock + threadIdx.x);
-                    s.join(v.x, v.y);
-                }
-                p.lse[query_row(p, rq, head, row)] = s.lse();
-            }
-            if (threadIdx.x == 0) *counter = 0;
-        }
-        __syncthreads();
-    }
-    if (bad != 0) record_page_fault(p.geo);
-}
-
-// Second pass: item = (request, KV head, 64 keys); the request's rows pass by in blocks of 64.
-template <typename T, int NC>
-__global__ __launch_bounds__(128) void weigh_sum_kernel(const WeighParams p) {
-    extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ float lse[2][kBlock];
-    await_previous_kernel();
-    const uint32_t count = p.scalars[kScalarWeighLong];
-    if (count == 0) return;
-    const WeighRequest* reqs = p.long_reqs();
-    const uint32_t total = reqs[count].cu1;
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, quad_row = lane >> 2, quad_col = lane & 3u;
-    const uint32_t chunks = p.geo.head_dim >> 3;
-    const uint32_t smem_base = uint32_t(__cvta_generic_to_shared(smem));
-    const PageBounds bounds(p.geo);
-    uint32_t bad = 0;
-    for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
-        const uint32_t r_index = find_request<1>(reqs, count, item);
-        const WeighRequest rq = reqs[r_index];
-        const uint32_t rows = rq.q_len * p.group, key_blocks = (rq.keys + kBlock - 1) / kBlock;
-        const uint32_t head = (item - rq.cu1) / key_blocks, key0 = (item - rq.cu1) % key_blocks * kBlock;
-        const uint32_t* row_ids = table_row(p.geo, rq.slot);
-        const uint32_t ka = key0 + warp * 16u + quad_row, kb = ka + 8u;
-        RowPair<NC> k;
-        load_row<NC>(k.lo, key_row(p, bounds, row_ids, head, min(ka, rq.keys - 1), bad), quad_col, chunks);
-        load_row<NC>(k.hi, key_row(p, bounds, row_ids, head, min(kb, rq.keys - 1), bad), quad_col, chunks);
-        // rows of tokens before the block's first key see none of it
-        const uint32_t row_begin = key0 > rq.first_pos ? (key0 - rq.first_pos) * p.group : 0u;
-        const auto fetch = [&](uint32_t row0, uint32_t stage) {
-#pragma unroll
-            for (uint32_t half = 0; half < 2; ++half) {
-                const uint32_t at = (threadIdx.x >> 2) + 32u * half, row = row0 + at;
-                const uint64_t q_row = query_row(p, rq, head, min(row, rows - 1));
-                copy_row<NC>(smem_base + stage * (kBlock * NC * 64u), at,
-                             reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + q_row * p.geo.head_dim), row < rows, chunks);
-                if ((threadIdx.x & 3u) == 0) lse[stage][at] = row < rows ? p.lse[q_row] : kInf;
-            }
-            cp_async_commit();
-        };
-        float sum0 = 0.0f, sum1 = 0.0f;
-        if (row_begin < rows) fetch(row_begin, 0);
-        uint32_t stage = 0;
-        for (uint32_t row0 = row_begin; row0 < rows; row0 += kBlock, stage ^= 1u) {
-            if (row0 + kBlock < rows) {
-                fetch(row0 + kBlock, stage ^ 1u);
-                cp_async_wait<1>();
-            } else {
-                cp_async_wait<0>();
-            }
-            __syncthreads();
-            float s[8][4];
-            block_product<T, NC>(s, k, smem + stage * (kBlock * NC * 64u), quad_row, quad_col);
-            const bool masked = key0 + kBlock > row_limit(p, rq, row0);
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const float2 n = *reinterpret_cast<const float2*>(&lse[stage][8 * t + 2 * quad_col]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float w = weight_of(s[t][e] * p.scale_log2, e & 1 ? n.y : n.x);
-                    if (masked && (e < 2 ? ka : kb) >= row_limit(p, rq, row0 + 8u * t + 2u * quad_col + (e & 1))) w = 0.0f;
-                    if (e < 2) sum0 += w;
-                    else sum1 += w;
-                }
-            }
-            __syncthreads();
-        }
-#pragma unroll
-        for (int x = 1; x < 4; x <<= 1) {
-            sum0 += __shfl_xor_sync(0xFFFFFFFFu, sum0, x);
-            sum1 += __shfl_xor_sync(0xFFFFFFFFu, sum1, x);
-        }
-        float* out = weight_row(p, rq, head);
-        if (quad_col == 0 && ka < rq.keys) out[ka] += sum0;
-        if (quad_col == 0 && kb < rq.keys) out[kb] += sum1;
-    }
-    if (bad != 0) record_page_fault(p.geo);
-}
-
 // ---- any type and head_dim: f32 products on the CUDA cores, 16 rows against 64 keys -----------------------------------------
 
-constexpr uint32_t kAnyRows = kWeighAnyRows;
+constexpr uint32_t kAnyRows = kWeighAnyRows, kBlock = kWeighAnyKeys;
 
 struct AnyTile {
     float* q;  // [16][d]
@@ -592,17 +328,18 @@ __global__ __launch_bounds__(128) void weigh_stats_any_kernel(const WeighParams 
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
                 const uint32_t row = row0 + at + a, limit = row < rows ? min(k1, row_limit(p, rq, row)) : 0u;
-                float m = st[a].m;
+                float m = -kInf;
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    s[a][b] = key0 + column + 16u * b < limit ? s[a][b] * p.scale_log2 : -kInf;
+                    s[a][b] = key0 + column + 16u * b < limit ? s[a][b] : -kInf;
                     m = fmaxf(m, s[a][b]);
                 }
+                m = fmaxf(st[a].m, m * p.scale_log2);
                 const float base = m == -kInf ? 0.0f : m;
-                st[a].l *= exp2f(st[a].m - base);
+                st[a].l *= exp2_approx(st[a].m - base);
                 st[a].m = m;
 #pragma unroll
-                for (int b = 0; b < 4; ++b) st[a].l += exp2f(s[a][b] - base);
+                for (int b = 0; b < 4; ++b) st[a].l += exp2_approx(fmaf(s[a][b], p.scale_log2, -base));
             }
             __syncthreads();
         }
@@ -615,7 +352,7 @@ __global__ __launch_bounds__(128) void weigh_stats_any_kernel(const WeighParams 
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
                 if (pieces == 1) {
-                    if (row0 + at + a < rows) p.lse[query_row(p, rq, head, row0 + at + a)] = st[a].lse();
+                    if (row0 + at + a < rows) p.norms[query_row(p, rq, head, row0 + at + a)] = st[a].norm();
                 } else {
                     p.long_partials()[uint64_t(item) * kAnyRows + at + a] = make_float2(st[a].m, st[a].l);
                 }
@@ -636,7 +373,7 @@ __global__ __launch_bounds__(128) void weigh_stats_any_kernel(const WeighParams 
                         const float2 v = __ldcg(p.long_partials() + uint64_t(rq.cu0 + unit * pieces + o) * kAnyRows + threadIdx.x);
                         s.join(v.x, v.y);
                     }
-                    p.lse[query_row(p, rq, head, row)] = s.lse();
+                    p.norms[query_row(p, rq, head, row)] = s.norm();
                 }
                 if (threadIdx.x == 0) *counter = 0;
             }
@@ -649,7 +386,7 @@ __global__ __launch_bounds__(128) void weigh_stats_any_kernel(const WeighParams 
 __global__ __launch_bounds__(128) void weigh_sum_any_kernel(const WeighParams p) {
     extern __shared__ __align__(16) float any_smem[];
     __shared__ float sums[8][kBlock];
-    __shared__ float lse[kAnyRows];
+    __shared__ float2 norms[kAnyRows];
     await_previous_kernel();
     const uint32_t count = p.scalars[kScalarWeighLong];
     if (count == 0) return;
@@ -668,7 +405,7 @@ __global__ __launch_bounds__(128) void weigh_sum_any_kernel(const WeighParams p)
         tile.load_keys(p, bounds, table_row(p.geo, rq.slot), head, key0, rq.keys, bad);
         for (uint32_t row0 = row_begin; row0 < rows; row0 += kAnyRows) {
             tile.load_rows(p, rq, head, row0, rows);
-            if (threadIdx.x < kAnyRows) lse[threadIdx.x] = row0 + threadIdx.x < rows ? p.lse[query_row(p, rq, head, row0 + threadIdx.x)] : kInf;
+            if (threadIdx.x < kAnyRows) norms[threadIdx.x] = row0 + threadIdx.x < rows ? p.norms[query_row(p, rq, head, row0 + threadIdx.x)] : make_float2(kInf, 0.0f);
             __syncthreads();
             float s[2][4];
             tile.product(s);
@@ -677,7 +414,7 @@ __global__ __launch_bounds__(128) void weigh_sum_any_kernel(const WeighParams p)
                 const uint32_t row = row0 + at + a, limit = row < rows ? row_limit(p, rq, row) : 0u;
 #pragma unroll
                 for (int b = 0; b < 4; ++b)
-                    if (key0 + column + 16u * b < limit) sum[b] += weight_of(s[a][b] * p.scale_log2, lse[at + a]);
+                    if (key0 + column + 16u * b < limit) sum[b] += weight_of(s[a][b], p.scale_log2, norms[at + a]);
             }
             __syncthreads();
         }
@@ -697,28 +434,19 @@ __global__ __launch_bounds__(128) void weigh_sum_any_kernel(const WeighParams p)
 
 template <typename T, int NC, int kMode>
 cudaError_t launch_short(const WeighParams& p, uint32_t ctas, cudaStream_t stream) {
-    return launch_overlapped(weigh_short_kernel<T, NC, kMode>, dim3(ctas), dim3(256), 0, stream, p);
+    constexpr int kSmem = 8 * 16 * NC * 64;
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(weigh_short_kernel<T, NC, kMode>), kSmem, done);
+    if (err != cudaSuccess) return err;
+    return launch_overlapped(weigh_short_kernel<T, NC, kMode>, dim3(ctas), dim3(256), kSmem, stream, p);
 }
 
 template <typename T, int NC>
 cudaError_t launch_tensor(const WeighParams& p, WeighPass pass, uint32_t ctas, cudaStream_t stream) {
-    constexpr int kSmem = 2 * kBlock * NC * 64;
     switch (pass) {
         case WeighPass::kShortStatsScores: return launch_short<T, NC, kStatsAndScores>(p, ctas, stream);
         case WeighPass::kShortStats: return launch_short<T, NC, kStatsOnly>(p, ctas, stream);
         case WeighPass::kShortSumAgain: return launch_short<T, NC, kSumAgain>(p, ctas, stream);
-        case WeighPass::kLongStats: {
-            static std::atomic<uint64_t> done{0};
-            const cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(weigh_stats_kernel<T, NC>), kSmem, done);
-            if (err != cudaSuccess) return err;
-            return launch_overlapped(weigh_stats_kernel<T, NC>, dim3(ctas), dim3(128), kSmem, stream, p);
-        }
-        case WeighPass::kLongSum: {
-            static std::atomic<uint64_t> done{0};
-            const cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(weigh_sum_kernel<T, NC>), kSmem, done);
-            if (err != cudaSuccess) return err;
-            return launch_overlapped(weigh_sum_kernel<T, NC>, dim3(ctas), dim3(128), kSmem, stream, p);
-        }
         default: return cudaErrorInvalidValue;
     }
 }
@@ -749,6 +477,7 @@ cudaError_t launch_any(const WeighParams& p, WeighPass pass, uint32_t ctas, cuda
 cudaError_t launch_weigh(const WeighParams& p, WeighPass pass, uint32_t ctas, cudaStream_t stream) {
     if (pass == WeighPass::kShortSumScores) return launch_overlapped(weigh_scores_kernel, dim3(ctas), dim3(256), 0, stream, p);
     if (!weigh_on_tensor_cores(p.dtype, p.geo.head_dim)) return launch_any(p, pass, ctas, stream);
+    if (pass == WeighPass::kLongStats || pass == WeighPass::kLongSum) return launch_weigh_umma(p, pass == WeighPass::kLongStats, ctas, stream);
     return p.dtype == PSI_DTYPE_BF16 ? launch_typed<__nv_bfloat16>(p, pass, ctas, stream) : launch_typed<__half>(p, pass, ctas, stream);
 }
 
