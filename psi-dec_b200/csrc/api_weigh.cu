@@ -115,7 +115,7 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
         const uint32_t block = tensor ? kWeighBlock : kWeighAnyRows;
         const bool can_short = tensor, can_long = !tensor || uint64_t(g->cfg.max_tokens) * group > kWeighShortRows;
         // one wave of the short-run kernel's workers
-        const uint64_t short_wave = sms * 2;
+        const uint64_t short_wave = sms;
         const uint64_t short_ctas = fixed ? (can_short ? short_wave : 0) : std::min<uint64_t>(short_wave, (w.tiles + 7) / 8);
         uint64_t short_units = uint64_t(w.num_short) * heads, long_units = w.long_units, stats_items = w.stats_items;
         if (fixed) {
@@ -152,6 +152,8 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
         p.counters = static_cast<uint32_t*>(w.counters.ptr);
         p.long_counters_at = short_units;
         p.group = group;
+        p.short_count = fixed ? 0xFFFFFFFFu : w.num_short;
+        p.short_tiles = fixed ? 0xFFFFFFFFu : static_cast<uint32_t>(w.tiles);
         p.num_q_heads = g->cfg.num_q_heads;
         p.dtype = g->cfg.dtype;
         p.scale_log2 = g->cfg.scale * 1.4426950408889634f;

@@ -14,16 +14,20 @@ __device__ __forceinline__ float exp2_approx(float x) {  // 2 ulp; results below
     return y;
 }
 
-// The request whose work holds `index`: the last one whose prefix (`which` 0: cu0, 1: cu1) is at or below it.
+// The request whose work holds `index`: the last one whose prefix (`which` 0: cu0, 1: cu1) is at or below it.  By a converged warp,
+// 32 requests at a time: a search that halves would wait for a load in each of its steps.
 template <int kWhich>
 __device__ __forceinline__ uint32_t find_request(const WeighRequest* reqs, uint32_t count, uint32_t index) {
-    uint32_t lo = 0, hi = count;  // invariant: prefix[lo] <= index < prefix[hi]
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if ((kWhich == 0 ? reqs[mid].cu0 : reqs[mid].cu1) <= index) lo = mid;
-        else hi = mid;
+    if (count == 1) return 0;
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t below = 0;
+#pragma unroll 4
+    for (uint32_t base = 0; base < count; base += 32) {
+        const uint32_t r = base + lane;
+        const uint32_t prefix = r < count ? (kWhich == 0 ? reqs[r].cu0 : reqs[r].cu1) : 0xFFFFFFFFu;
+        below += __popc(__ballot_sync(0xFFFFFFFFu, r < count && prefix <= index));
     }
-    return lo;
+    return below - 1;
 }
 
 // (maximum, sum) of a row's scores in the log2 domain; an empty one is (-inf, 0).

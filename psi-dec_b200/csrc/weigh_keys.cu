@@ -9,12 +9,13 @@
 // M and 1 / L stay apart: their logarithmic sum is a number of twenty or so, whose rounding alone would be the largest error.
 //
 //   weigh_short_kernel   runs of up to 16 rows (decode, drafts): bound by the K bytes.  One warp is one worker with an equal
-//                        share of the batch's 32-key tiles.  Products do not depend on the order of the columns of q and k, so
-//                        a lane takes 16 consecutive bytes of a key row as the operands of two m16n8k16 steps, and the
-//                        same bytes of the query rows (from shared memory): K goes from HBM to registers with no barrier, for any
-//                        page size.  The first pass leaves its scores in scratch, 4 bytes a row and key against 2 head_dim
-//                        bytes a key, so that K is read once; where there is no scratch (captured launches, very
-//                        large batches) the second pass reads K again.
+//                        share of the batch's 32-key tiles, which it streams through a ring of its own (cp.async, no barrier
+//                        of the CTA; any page size), page IDs fetched a step ahead of the keys, which are two to eleven ahead of their
+//                        use.  Products do not depend on the order of the columns of q and k, so a lane takes 16 consecutive
+//                        bytes of a key row as the operands of two m16n8k16 steps, and the same bytes of the query rows, which
+//                        stay in registers.  The first pass leaves its products in scratch, 4 bytes a row and key against
+//                        2 head_dim bytes a key, so that K is read once; where there is no scratch (captured launches,
+//                        very large batches) the second pass reads K again.
 //   weigh_umma_kernel    longer runs, on tcgen05 (weigh_umma.cu).
 //   weigh_*_any_kernel   f32 and head dims that are no multiple of eight: the same two passes in f32 on the CUDA cores.
 #include "mma_common.cuh"
@@ -58,24 +59,89 @@ __device__ __forceinline__ uint32_t block_offset(uint32_t row, uint32_t chunk) {
 
 enum ShortMode { kStatsAndScores = 0, kStatsOnly = 1, kSumAgain = 2 };
 
+// Steps of 16 keys that a warp's ring holds: 24 KiB a warp, 192 KiB an SM.
+template <int NC>
+constexpr int kRingSteps = 24 / NC;
+
+// Requests and tiles of the short runs: with the launch where the host knows them, which spares two loads one behind the other.
+struct ShortWork {
+    uint32_t count, total;
+    __device__ __forceinline__ explicit ShortWork(const WeighParams& p) : count(p.short_count), total(p.short_tiles) {
+        if (count == 0xFFFFFFFFu) {
+            count = p.scalars[kScalarWeighShort];
+            total = p.reqs[count].cu0;
+        }
+    }
+};
+
 template <typename T, int NC, int kMode>
-__global__ __launch_bounds__(256, 2) void weigh_short_kernel(const WeighParams p) {
+__global__ __launch_bounds__(256, 1) void weigh_short_kernel(const WeighParams p) {
+    constexpr uint32_t kStepBytes = 16 * NC * 64;
+    constexpr int kSteps = kRingSteps<NC>;
     extern __shared__ __align__(128) unsigned char smem[];
     await_previous_kernel();
-    const uint32_t count = p.scalars[kScalarWeighShort];
-    if (count == 0) return;
+    const ShortWork work(p);
+    const uint32_t count = work.count, total = work.total;
     const WeighRequest* reqs = p.reqs;
-    const uint32_t total = reqs[count].cu0;
     const uint32_t workers = min(gridDim.x * 8u, total);
     const uint32_t w = blockIdx.x * 8u + (threadIdx.x >> 5);
     if (w >= workers) return;
-    unsigned char* q_rows = smem + (threadIdx.x >> 5) * (16 * NC * 64);  // this warp's
+    const unsigned char* ring = smem + (threadIdx.x >> 5) * (kSteps * kStepBytes);  // this warp's
+    const uint32_t ring_at = uint32_t(__cvta_generic_to_shared(ring));
     const uint32_t lane = threadIdx.x & 31u, quad_row = lane >> 2, quad_col = lane & 3u;
     const uint32_t begin = uint32_t(uint64_t(w) * total / workers), end = uint32_t(uint64_t(w + 1) * total / workers);
     const uint32_t chunks = p.geo.head_dim >> 3;
+    const uint64_t policy = l2_evict_first_policy();
     const PageBounds bounds(p.geo);
     uint32_t bad = 0;
     uint32_t r_index = find_request<0>(reqs, count, begin);
+    // The load cursor: a step of 16 keys, whose page IDs (of row lane % 16) are fetched a step before its keys.
+    uint32_t load_step = 0, id_tile = begin, id_half = 0, id_request = r_index, id_head = 0, id_next = begin, id_begin = 0;
+    const uint32_t* id_rows = nullptr;
+    uint32_t id_keys = 0, page = 0, page_token = 0, page_head = 0;
+    bool more = true;
+    const auto fetch_ids = [&] {
+        if (id_tile >= end) {
+            more = false;
+            return;
+        }
+        if (id_tile >= id_next) {  // another (request, KV head)
+            while (reqs[id_request + 1].cu0 <= id_tile) ++id_request;
+            const WeighRequest rq = reqs[id_request];
+            const uint32_t per_head = (rq.keys + 31u) / 32u;
+            id_head = (id_tile - rq.cu0) / per_head;
+            id_begin = rq.cu0 + id_head * per_head;
+            id_next = id_begin + per_head;
+            id_keys = rq.keys;
+            id_rows = table_row(p.geo, rq.slot);
+        }
+        const uint32_t key = min((id_tile - id_begin) * 32u + id_half * 16u + (lane & 15u), id_keys - 1u);
+        page = bounds.read(id_rows, key / p.geo.tokens_per_page, bad);
+        page_token = key % p.geo.tokens_per_page;
+        page_head = id_head;
+        if (id_half != 0) ++id_tile;
+        id_half ^= 1u;
+    };
+    const auto load_next = [&] {
+        if (more) {
+            const uint64_t offset = kv_row_offset(p.geo, page, page_head, page_token);  // of row lane % 16
+            const uint32_t dst = ring_at + (load_step % kSteps) * kStepBytes;
+#pragma unroll
+            for (int j = 0; j < 2 * NC; ++j) {
+                const uint32_t at = lane + 32u * j, row = at / (NC * 4u), c = at % (NC * 4u);
+                const uint64_t from = __shfl_sync(0xFFFFFFFFu, offset, row);
+                const bool live = c < chunks;
+                cp_async_16_hinted(dst + block_offset<NC>(row, c), static_cast<const uint16_t*>(p.geo.pages) + from + (live ? c * 8u : 0u), live ? 16u : 0u, policy);
+            }
+            ++load_step;
+            fetch_ids();
+        }
+        cp_async_commit();
+    };
+    fetch_ids();
+#pragma unroll 1
+    for (int i = 0; i < kSteps - 1; ++i) load_next();
+    uint32_t step = 0;
     for (uint32_t tile = begin; tile < end;) {
         while (reqs[r_index + 1].cu0 <= tile) ++r_index;
         const WeighRequest rq = reqs[r_index];
@@ -84,21 +150,11 @@ __global__ __launch_bounds__(256, 2) void weigh_short_kernel(const WeighParams p
         const uint32_t unit_begin = rq.cu0 + head * per_head, unit_end = unit_begin + per_head;
         const uint32_t last = min(end, unit_end);
         const uint32_t rows = rq.q_len * p.group;
-        const uint32_t* row_ids = table_row(p.geo, rq.slot);
-        // the unit's query rows, zeros behind them
-        __syncwarp();
+        uint4 q_lo[NC], q_hi[NC];
 #pragma unroll
-        for (uint32_t half = 0; half < 2; ++half) {
-            const uint32_t row = quad_row + 8 * half;
-            uint4 x[NC];
-#pragma unroll
-            for (int i = 0; i < NC; ++i) x[i] = make_uint4(0, 0, 0, 0);
-            if (row < rows)
-                load_row<NC>(x, reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + query_row(p, rq, head, row) * p.geo.head_dim), quad_col, chunks);
-#pragma unroll
-            for (int i = 0; i < NC; ++i) *reinterpret_cast<uint4*>(q_rows + block_offset<NC>(row, quad_col + 4u * i)) = x[i];
-        }
-        __syncwarp();
+        for (int i = 0; i < NC; ++i) q_lo[i] = q_hi[i] = make_uint4(0, 0, 0, 0);
+        if (quad_row < rows) load_row<NC>(q_lo, reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + query_row(p, rq, head, quad_row) * p.geo.head_dim), quad_col, chunks);
+        if (quad_row + 8 < rows) load_row<NC>(q_hi, reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + query_row(p, rq, head, quad_row + 8) * p.geo.head_dim), quad_col, chunks);
         const bool two_halves = rows > 8;
         const uint32_t limit0 = quad_row < rows ? row_limit(p, rq, quad_row) : 0u;
         const uint32_t limit1 = quad_row + 8 < rows ? row_limit(p, rq, quad_row + 8) : 0u;
@@ -108,39 +164,34 @@ __global__ __launch_bounds__(256, 2) void weigh_short_kernel(const WeighParams p
             if (quad_row < rows) norm0 = p.norms[query_row(p, rq, head, quad_row)];
             if (quad_row + 8 < rows) norm1 = p.norms[query_row(p, rq, head, quad_row + 8)];
         }
-        constexpr int kBatch = NC <= 4 ? 4 : 2;  // 8-key groups whose rows are in flight at once
         for (; tile < last; ++tile) {
-            const uint32_t key0 = (tile - unit_begin) * 32u;
+#pragma unroll 1
+            for (uint32_t half = 0; half < 2; ++half, ++step) {
+                const uint32_t key0 = (tile - unit_begin) * 32u + half * 16u;
+                cp_async_wait<kSteps - 2>();
+                __syncwarp();  // the step's keys have landed, and everyone is through with the step before it, whose place is next
+                load_next();
+                const unsigned char* k = ring + (step % kSteps) * kStepBytes;
+                float s[2][4];  // products, -inf where a row does not see a key
 #pragma unroll
-            for (int half = 0; half < 4; half += kBatch) {
-                uint4 k[kBatch][NC];
-#pragma unroll
-                for (int t = 0; t < kBatch; ++t) {
-                    const uint32_t key = min(key0 + 8u * (half + t) + quad_row, rq.keys - 1u);
-                    load_row<NC>(k[t], key_row(p, bounds, row_ids, head, key, bad), quad_col, chunks);
-                }
-                float s[kBatch][4];  // products, -inf where a row does not see a key
-#pragma unroll
-                for (int t = 0; t < kBatch; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
+                for (int t = 0; t < 2; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < NC; ++i) {
-                    const uint4 lo = *reinterpret_cast<const uint4*>(q_rows + block_offset<NC>(quad_row, quad_col + 4u * i));
-                    uint4 hi = make_uint4(0, 0, 0, 0);
-                    if (two_halves) hi = *reinterpret_cast<const uint4*>(q_rows + block_offset<NC>(quad_row + 8, quad_col + 4u * i));
 #pragma unroll
-                    for (int t = 0; t < kBatch; ++t) chunk_mma<T>(s[t], lo, hi, k[t][i]);
+                    for (int t = 0; t < 2; ++t)
+                        chunk_mma<T>(s[t], q_lo[i], q_hi[i], *reinterpret_cast<const uint4*>(k + block_offset<NC>(8u * t + quad_row, quad_col + 4u * i)));
                 }
 #pragma unroll
-                for (int t = 0; t < kBatch; ++t) {
+                for (int t = 0; t < 2; ++t) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const uint32_t key = key0 + 8u * (half + t) + 2u * quad_col + (e & 1);
+                        const uint32_t key = key0 + 8u * t + 2u * quad_col + (e & 1);
                         s[t][e] = key < (e < 2 ? limit0 : limit1) ? s[t][e] : -kInf;
                     }
                 }
                 if (kMode == kSumAgain) {
 #pragma unroll
-                    for (int t = 0; t < kBatch; ++t) {
+                    for (int t = 0; t < 2; ++t) {
                         float a = weight_of(s[t][0], p.scale_log2, norm0) + weight_of(s[t][2], p.scale_log2, norm1);
                         float b = weight_of(s[t][1], p.scale_log2, norm0) + weight_of(s[t][3], p.scale_log2, norm1);
 #pragma unroll
@@ -148,7 +199,7 @@ __global__ __launch_bounds__(256, 2) void weigh_short_kernel(const WeighParams p
                             a += __shfl_xor_sync(0xFFFFFFFFu, a, x);
                             b += __shfl_xor_sync(0xFFFFFFFFu, b, x);
                         }
-                        const uint32_t key = key0 + 8u * (half + t) + 2u * quad_col;
+                        const uint32_t key = key0 + 8u * t + 2u * quad_col;
                         float* row = weight_row(p, rq, head);
                         if (quad_row == 0 && key < rq.keys) row[key] += a;
                         if (quad_row == 0 && key + 1 < rq.keys) row[key + 1] += b;
@@ -157,29 +208,27 @@ __global__ __launch_bounds__(256, 2) void weigh_short_kernel(const WeighParams p
                     if (kMode == kStatsAndScores) {
                         // [8-key group][row][8 keys], as many rows as the batch's longest run has
 #pragma unroll
-                        for (int t = 0; t < kBatch; ++t) {
-                            float* at = p.scores + (uint64_t(tile) * 4u + half + t) * 8u * p.score_rows + quad_row * 8u + 2u * quad_col;
+                        for (int t = 0; t < 2; ++t) {
+                            float* at = p.scores + (uint64_t(tile) * 4u + half * 2 + t) * 8u * p.score_rows + quad_row * 8u + 2u * quad_col;
                             if (quad_row < p.score_rows) *reinterpret_cast<float2*>(at) = make_float2(s[t][0], s[t][1]);
                             if (quad_row + 8 < p.score_rows) *reinterpret_cast<float2*>(at + 64) = make_float2(s[t][2], s[t][3]);
                         }
                     }
-                    float m0 = -kInf, m1 = -kInf;
-#pragma unroll
-                    for (int t = 0; t < kBatch; ++t) {
-                        m0 = fmaxf(m0, fmaxf(s[t][0], s[t][1]));
-                        m1 = fmaxf(m1, fmaxf(s[t][2], s[t][3]));
-                    }
-                    m0 = fmaxf(s0.m, m0 * p.scale_log2);
-                    m1 = fmaxf(s1.m, m1 * p.scale_log2);
-                    const float base0 = m0 == -kInf ? 0.0f : m0, base1 = m1 == -kInf ? 0.0f : m1;
+                    const float m0 = fmaxf(s0.m, fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])) * p.scale_log2);
+                    const float base0 = m0 == -kInf ? 0.0f : m0;
                     s0.l *= exp2_approx(s0.m - base0);
-                    s1.l *= exp2_approx(s1.m - base1);
                     s0.m = m0;
-                    s1.m = m1;
 #pragma unroll
-                    for (int t = 0; t < kBatch; ++t) {
+                    for (int t = 0; t < 2; ++t)
                         s0.l += exp2_approx(fmaf(s[t][0], p.scale_log2, -base0)) + exp2_approx(fmaf(s[t][1], p.scale_log2, -base0));
-                        if (two_halves) s1.l += exp2_approx(fmaf(s[t][2], p.scale_log2, -base1)) + exp2_approx(fmaf(s[t][3], p.scale_log2, -base1));
+                    if (two_halves) {
+                        const float m1 = fmaxf(s1.m, fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])) * p.scale_log2);
+                        const float base1 = m1 == -kInf ? 0.0f : m1;
+                        s1.l *= exp2_approx(s1.m - base1);
+                        s1.m = m1;
+#pragma unroll
+                        for (int t = 0; t < 2; ++t)
+                            s1.l += exp2_approx(fmaf(s[t][2], p.scale_log2, -base1)) + exp2_approx(fmaf(s[t][3], p.scale_log2, -base1));
                     }
                 }
             }
@@ -212,13 +261,18 @@ __global__ __launch_bounds__(256, 2) void weigh_short_kernel(const WeighParams p
         arrived = __shfl_sync(0xFFFFFFFFu, arrived, 0);
         if (arrived == last_worker - first_worker) {
             __threadfence();
+            // lanes: rows, and workers of the unit side by side; eight loads under way at a time
+            const uint32_t wide = rows > 8 ? 16u : 8u, row = lane & (wide - 1), beside = 32u / wide;
             Stat s{-kInf, 0.0f};
-            const uint32_t row = lane & 15u;
-            for (uint32_t o = first_worker + (lane >> 4); o <= last_worker; o += 2) {
-                const float2 v = __ldcg(p.partials + uint64_t(o + unit) * 16u + row);
-                s.join(v.x, v.y);
+            for (uint32_t o = first_worker + lane / wide; o <= last_worker; o += 8 * beside) {
+                float2 v[8];
+#pragma unroll
+                for (uint32_t x = 0; x < 8; ++x)
+                    v[x] = o + x * beside <= last_worker ? __ldcg(p.partials + uint64_t(o + x * beside + unit) * 16u + row) : make_float2(-kInf, 0.0f);
+#pragma unroll
+                for (uint32_t x = 0; x < 8; ++x) s.join(v[x].x, v[x].y);
             }
-            s.join(__shfl_xor_sync(0xFFFFFFFFu, s.m, 16), __shfl_xor_sync(0xFFFFFFFFu, s.l, 16));
+            for (uint32_t x = wide; x < 32; x <<= 1) s.join(__shfl_xor_sync(0xFFFFFFFFu, s.m, x), __shfl_xor_sync(0xFFFFFFFFu, s.l, x));
             if (lane < rows) p.norms[query_row(p, rq, head, lane)] = s.norm();
             if (lane == 0) p.counters[unit] = 0;
         }
@@ -229,27 +283,43 @@ __global__ __launch_bounds__(256, 2) void weigh_short_kernel(const WeighParams p
 // Second pass over stored scores: a lane is a key.
 __global__ __launch_bounds__(256) void weigh_scores_kernel(const WeighParams p) {
     await_previous_kernel();
-    const uint32_t count = p.scalars[kScalarWeighShort];
-    if (count == 0) return;
+    const ShortWork work(p);
     const WeighRequest* reqs = p.reqs;
-    const uint32_t total = reqs[count].cu0;
-    const uint32_t workers = min(gridDim.x * 8u, total);
+    const uint32_t workers = min(gridDim.x * 8u, work.total);
     const uint32_t w = blockIdx.x * 8u + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
     if (w >= workers) return;
-    const uint32_t begin = uint32_t(uint64_t(w) * total / workers), end = uint32_t(uint64_t(w + 1) * total / workers);
-    uint32_t r_index = find_request<0>(reqs, count, begin);
+    const uint32_t begin = uint32_t(uint64_t(w) * work.total / workers), end = uint32_t(uint64_t(w + 1) * work.total / workers);
+    const uint32_t first = find_request<0>(reqs, work.count, begin);
+    uint32_t r_index = first, unit_end = 0, unit_begin = 0, head = 0;
+    WeighRequest rq{};
+    uint32_t rows = 0;
+    float2 norm = make_float2(0.0f, 0.0f);  // of row `lane`
     for (uint32_t tile = begin; tile < end; ++tile) {
-        while (reqs[r_index + 1].cu0 <= tile) ++r_index;
-        const WeighRequest rq = reqs[r_index];
-        const uint32_t per_head = (rq.keys + 31u) / 32u;
-        const uint32_t head = (tile - rq.cu0) / per_head;
-        const uint32_t key = (tile - rq.cu0 - head * per_head) * 32u + lane;
-        const uint32_t rows = rq.q_len * p.group;
+        float product[kWeighShortRows];
         const float* s = p.scores + (uint64_t(tile) * 4u + (lane >> 3)) * 8u * p.score_rows + (lane & 7u);
+#pragma unroll
+        for (uint32_t r = 0; r < kWeighShortRows; ++r)
+            if (r < p.score_rows) product[r] = __ldcs(s + r * 8u);
+        if (tile >= unit_end) {  // another (request, KV head)
+            while (reqs[r_index + 1].cu0 <= tile) ++r_index;
+            rq = reqs[r_index];
+            const uint32_t per_head = (rq.keys + 31u) / 32u;
+            head = (tile - rq.cu0) / per_head;
+            unit_begin = rq.cu0 + head * per_head;
+            unit_end = unit_begin + per_head;
+            rows = rq.q_len * p.group;
+            norm = lane < rows ? p.norms[query_row(p, rq, head, lane)] : make_float2(kInf, 0.0f);
+        }
+        const uint32_t key = (tile - unit_begin) * 32u + lane;
+        float* at = weight_row(p, rq, head) + key;
+        const float before = key < rq.keys ? *at : 0.0f;
         float sum = 0.0f;
-        #pragma unroll 4
-        for (uint32_t r = 0; r < rows; ++r) sum += weight_of(s[r * 8u], p.scale_log2, p.norms[query_row(p, rq, head, r)]);
-        if (key < rq.keys) weight_row(p, rq, head)[key] += sum;
+#pragma unroll
+        for (uint32_t r = 0; r < kWeighShortRows; ++r) {
+            const float2 of_row = make_float2(__shfl_sync(0xFFFFFFFFu, norm.x, r), __shfl_sync(0xFFFFFFFFu, norm.y, r));
+            if (r < p.score_rows) sum += weight_of(product[r], p.scale_log2, of_row);
+        }
+        if (key < rq.keys) *at = before + sum;
     }
 }
 
@@ -434,7 +504,7 @@ __global__ __launch_bounds__(128) void weigh_sum_any_kernel(const WeighParams p)
 
 template <typename T, int NC, int kMode>
 cudaError_t launch_short(const WeighParams& p, uint32_t ctas, cudaStream_t stream) {
-    constexpr int kSmem = 8 * 16 * NC * 64;
+    constexpr int kSmem = 8 * kRingSteps<NC> * 16 * NC * 64;
     static std::atomic<uint64_t> done{0};
     const cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(weigh_short_kernel<T, NC, kMode>), kSmem, done);
     if (err != cudaSuccess) return err;

@@ -55,6 +55,7 @@ struct WeighParams {
     uint64_t stride;
     const WeighRequest* reqs;
     const uint32_t* scalars;
+    uint32_t short_count, short_tiles;  // requests and tiles of the short runs, or ~0: as the device block says (captured launches)
     float2* norms;                // [max_tokens][Hq] log2-domain maximum and 1 / sum of each row; (inf, 0) for a row that adds nothing
     float2* partials;             // (m, l) by segment of the short runs, then by item of the long ones
     uint64_t long_partials_at;
