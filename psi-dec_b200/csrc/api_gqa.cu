@@ -75,6 +75,7 @@ int32_t psi_gqa_destroy(psi_gqa* g) {
         g->weigh.partials.release();
         g->weigh.counters.release();
         g->weigh.scores.release();
+        g->weigh.sums.release();
         for (cudaEvent_t e : g->pipe_events) (void)cudaEventDestroy(e);
         if (g->pipe_h2d != nullptr) (void)cudaStreamDestroy(g->pipe_h2d);
         if (g->pipe_d2h != nullptr) (void)cudaStreamDestroy(g->pipe_d2h);

@@ -198,10 +198,11 @@ struct psi_weigh_plan {
     uint64_t tiles = 0, stats_items = 0, sum_items = 0, long_units = 0;
     bool repeated = false;               // a slot appears twice in the batch
     bool too_large = false;
+    bool parted = false;                 // rows of a long run are cut into parts in the second pass
     bool captured = false;               // a captured launch sequence holds key-weight launches
     std::vector<uint32_t> seen;          // by slot: the epoch that last named it
     uint32_t epoch = 0;
-    psi::DeviceBuffer norms, partials, counters, scores;
+    psi::DeviceBuffer norms, partials, counters, scores, sums;
 };
 
 struct psi_gqa {

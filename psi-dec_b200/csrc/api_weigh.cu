@@ -14,7 +14,7 @@ void plan_weigh(psi_gqa* g, const uint32_t* req_slots, const uint32_t* token_ind
     w.reqs.clear();
     w.num_short = w.num_long = w.max_keys = w.short_rows = 0;
     w.long_units = 0;
-    w.repeated = w.too_large = false;
+    w.repeated = w.too_large = w.parted = false;
     const uint32_t group = g->cfg.num_q_heads / g->cfg.num_kv_heads, heads = g->cfg.num_kv_heads;
     const bool tensor = weigh_on_tensor_cores(g->cfg.dtype, g->cfg.head_dim);
     const uint32_t block = tensor ? kWeighBlock : kWeighAnyRows;
@@ -47,8 +47,10 @@ void plan_weigh(psi_gqa* g, const uint32_t* req_slots, const uint32_t* token_ind
                 w.num_long += 1;
                 const uint64_t units = (rows + block - 1) / block * heads;
                 w.long_units += units;
-                cu0 += units * weigh_pieces(keys);
-                cu1 += weigh_sum_items(keys, tensor) * heads;
+                cu0 += units * weigh_pieces(keys, tensor);
+                const uint64_t parts = g->replay_reserved ? 1 : weigh_row_parts(static_cast<uint32_t>(std::min<uint64_t>(rows, kU32Max)), keys, heads, tensor);
+                if (parts > 1) w.parted = true;
+                cu1 += parts * weigh_spans(keys, tensor) * heads;
             }
         }
         WeighRequest end{};
@@ -122,11 +124,13 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
             short_units = can_short ? uint64_t(g->cfg.max_tokens) * heads : 0;
             const uint64_t rows = uint64_t(g->cfg.max_tokens) * group;
             long_units = can_long ? (rows / block + (tensor ? rows / (kWeighShortRows + 1) : g->cfg.max_tokens) + 1) * heads : 0;
-            stats_items = long_units * weigh_pieces(static_cast<uint32_t>(std::min<uint64_t>(table_tokens(g), kU32Max)));
+            stats_items = long_units * weigh_pieces(static_cast<uint32_t>(std::min<uint64_t>(table_tokens(g), kU32Max)), tensor);
         }
         const uint64_t short_slots = (short_ctas * 8 + short_units) * 16, long_slots = stats_items * block;
         const uint64_t partial_bytes = (short_slots + long_slots) * sizeof(float2);
-        const uint64_t counter_words = short_units + long_units;
+        // (a span's counter stands at the place of its first item)
+        const uint64_t counter_words = short_units + std::max(long_units, w.parted ? w.sum_items : 0);
+        const uint64_t sum_bytes = w.parted ? w.sum_items * weigh_span_keys(tensor) * sizeof(float) : 0;
         if (ctx->capturing) {
             require(w.norms.ptr != nullptr && partial_bytes <= w.partials.bytes && counter_words * sizeof(uint32_t) <= w.counters.bytes,
                     "call psi_gqa_weigh_keys once after the replay reservation and before the capture: it allocates its scratch then");
@@ -136,6 +140,7 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
                     "the largest batch the replayed steps carry");
             w.norms.ensure(ctx, uint64_t(g->cfg.max_tokens) * g->cfg.num_q_heads * sizeof(float2), false);
             w.partials.ensure(ctx, partial_bytes > w.partials.bytes ? std::max<uint64_t>(partial_bytes * 3 / 2, 1 << 16) : partial_bytes, false);
+            w.sums.ensure(ctx, sum_bytes > w.sums.bytes ? sum_bytes * 3 / 2 : sum_bytes, false);
             if (counter_words * sizeof(uint32_t) > w.counters.bytes) {
                 w.counters.release_after(ctx);  // counters restart from zero at their new size
                 w.counters.ensure(ctx, std::max<uint64_t>(counter_words * 6, 1 << 12), true);
@@ -151,6 +156,8 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
         p.long_partials_at = short_slots;
         p.counters = static_cast<uint32_t*>(w.counters.ptr);
         p.long_counters_at = short_units;
+        p.sums = static_cast<float*>(w.sums.ptr);
+        p.split_rows = fixed ? 0u : 1u;
         p.group = group;
         p.short_count = fixed ? 0xFFFFFFFFu : w.num_short;
         p.short_tiles = fixed ? 0xFFFFFFFFu : static_cast<uint32_t>(w.tiles);
@@ -175,7 +182,7 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
         }
         if (ctx->capturing) w.captured = true;
         if (short_ctas > 0) run_pass(g, p, keep_scores ? WeighPass::kShortStatsScores : WeighPass::kShortStats, short_ctas);
-        const uint64_t long_wave = sms * (tensor ? 2 : 8);
+        const uint64_t long_wave = sms * (tensor || g->cfg.head_dim > 96 ? 2 : 4);
         const uint64_t stats_ctas = fixed ? (can_long ? long_wave : 0) : std::min<uint64_t>(long_wave, w.stats_items);
         const uint64_t sum_ctas = fixed ? stats_ctas : std::min<uint64_t>(long_wave, w.sum_items);
         if (stats_ctas > 0) run_pass(g, p, WeighPass::kLongStats, stats_ctas);

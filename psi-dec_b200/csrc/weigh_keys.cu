@@ -323,51 +323,96 @@ __global__ __launch_bounds__(256) void weigh_scores_kernel(const WeighParams p) 
     }
 }
 
-// ---- any type and head_dim: f32 products on the CUDA cores, 16 rows against 64 keys -----------------------------------------
+// ---- any type and head_dim: f32 products on the CUDA cores, 32 rows against 64 keys -----------------------------------------
 
 constexpr uint32_t kAnyRows = kWeighAnyRows, kBlock = kWeighAnyKeys;
+constexpr uint32_t kAnyThreads = kAnyRows / 2 * 16;  // two rows and four keys each
+
+// Rows and keys in shared memory as f32, an odd number of 16-byte units apart, so that 16-byte reads of neighbouring keys
+// fall into distinct banks; two key blocks, the next one under way while one is worked on (f32 with head_dim a multiple of four
+// and 16-byte boundaries, `wide`: by cp.async; everything else element by element).
+// Floats from one row to the next: an odd multiple of four.
+__host__ __device__ inline uint32_t any_pitch(uint32_t head_dim) { return ((head_dim + 3) / 4 | 1u) * 4u; }
 
 struct AnyTile {
-    float* q;  // [16][d]
-    float* k;  // [64][d + 1]
-    uint32_t d;
-    __device__ __forceinline__ AnyTile(float* smem, uint32_t head_dim) : q(smem), k(smem + kAnyRows * head_dim), d(head_dim) {}
-    __device__ __forceinline__ void load_rows(const WeighParams& p, const WeighRequest& rq, uint32_t head, uint32_t row0, uint32_t rows) {
-        for (uint32_t i = threadIdx.x; i < kAnyRows * d; i += blockDim.x) {
-            const uint32_t row = row0 + i / d;
-            q[i] = row < rows ? load_as_float(p.q, query_row(p, rq, head, row) * d + i % d, p.dtype) : 0.0f;
+    float* q;
+    float* k[2];
+    uint32_t d, pitch;
+    bool wide;
+    __device__ __forceinline__ AnyTile(float* smem, const WeighParams& p)
+        : d(p.geo.head_dim), pitch(any_pitch(p.geo.head_dim)),
+          wide(p.dtype == PSI_DTYPE_F32 && p.geo.head_dim % 4 == 0 && ((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.geo.pages)) & 15u) == 0) {
+        q = smem;
+        k[0] = q + kAnyRows * pitch;
+        k[1] = k[0] + kBlock * pitch;
+        if (d % 4 != 0) {  // the elements that pad a row to a multiple of four take part in the products
+            for (uint32_t row = threadIdx.x; row < kAnyRows + 2 * kBlock; row += blockDim.x)
+                for (uint32_t i = d; i < pitch; ++i) smem[row * pitch + i] = 0.0f;
+            __syncthreads();
         }
     }
-    __device__ __forceinline__ void load_keys(const WeighParams& p, const PageBounds& bounds, const uint32_t* row_ids, uint32_t head,
-                                              uint32_t key0, uint32_t keys, uint32_t& bad) {
-        for (uint32_t at = threadIdx.x >> 5; at < kBlock; at += blockDim.x >> 5) {
-            const uint32_t key = key0 + at;
-            if (key >= keys) continue;  // never read: those columns are masked
-            const uint32_t page = bounds.read(row_ids, key / p.geo.tokens_per_page, bad);
-            const uint64_t row = kv_row_offset(p.geo, page, head, key % p.geo.tokens_per_page);
-            for (uint32_t i = threadIdx.x & 31u; i < d; i += 32u) k[at * (d + 1) + i] = load_as_float(p.geo.pages, row + i, p.dtype);
+    __device__ __forceinline__ void load_rows(float* to, const WeighParams& p, const WeighRequest& rq, uint32_t head, uint32_t row0, uint32_t rows) const {
+        for (uint32_t at = threadIdx.x >> 5; at < kAnyRows; at += blockDim.x >> 5) {
+            const uint32_t row = row0 + at;
+            const uint64_t from = row < rows ? query_row(p, rq, head, row) * d : 0u;
+            if (wide) {
+                const uint32_t dst = uint32_t(__cvta_generic_to_shared(to + at * pitch));
+                for (uint32_t i = 4 * (threadIdx.x & 31u); i < d; i += 128u) cp_async_16(dst + i * 4, static_cast<const float*>(p.q) + from + i, row < rows ? 16u : 0u);
+            } else {
+                for (uint32_t i = threadIdx.x & 31u; i < d; i += 32u) to[at * pitch + i] = row < rows ? load_as_float(p.q, from + i, p.dtype) : 0.0f;
+            }
         }
+    }
+    __device__ __forceinline__ void load_keys(uint32_t stage, const WeighParams& p, const PageBounds& bounds, const uint32_t* row_ids, uint32_t head,
+                                              uint32_t key0, uint32_t keys, uint32_t& bad) const {
+        // rows at and beyond `keys` keep what they hold: those columns are masked
+        const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+        constexpr uint32_t kEach = kBlock / (kAnyThreads / 32);  // of a warp
+        const uint32_t mine = key0 + warp * kEach + (lane & (kEach - 1));
+        uint64_t offset = 0;
+        if (mine < keys) offset = kv_row_offset(p.geo, bounds.read(row_ids, mine / p.geo.tokens_per_page, bad), head, mine % p.geo.tokens_per_page);
+        if (wide) {
+            // as many lanes as a row has 16-byte units take one
+            const uint32_t units = d / 4, lanes = units >= 32 ? 32u : units > 8 ? 16u : 8u, beside = 32u / lanes;
+            for (uint32_t at = 0; at < kEach; at += beside) {
+                const uint32_t r = at + lane / lanes;
+                const uint64_t from = __shfl_sync(0xFFFFFFFFu, offset, r);
+                const uint32_t dst = uint32_t(__cvta_generic_to_shared(k[stage] + (warp * kEach + r) * pitch));
+                if (key0 + warp * kEach + r < keys)
+                    for (uint32_t u = lane % lanes; u < units; u += lanes) cp_async_16(dst + u * 16, static_cast<const float*>(p.geo.pages) + from + u * 4, 16u);
+            }
+        } else {
+            for (uint32_t r = 0; r < kEach; ++r) {
+                const uint64_t from = __shfl_sync(0xFFFFFFFFu, offset, r);
+                if (key0 + warp * kEach + r < keys)
+                    for (uint32_t i = lane; i < d; i += 32u) k[stage][(warp * kEach + r) * pitch + i] = load_as_float(p.geo.pages, from + i, p.dtype);
+            }
+        }
+        cp_async_commit();
     }
     // Thread t: rows 2 (t / 16) + {0, 1}, keys t % 16 + 16 {0..3}.
-    __device__ __forceinline__ void product(float (&s)[2][4]) const {
-        const uint32_t row = 2u * (threadIdx.x >> 4), key = threadIdx.x & 15u;
+    __device__ __forceinline__ void product(const float* rows, uint32_t stage, float (&s)[2][4]) const {
+        const float4* q0 = reinterpret_cast<const float4*>(rows + 2u * (threadIdx.x >> 4) * pitch);
+        const float4* q1 = q0 + pitch / 4;
+        const float4* x = reinterpret_cast<const float4*>(k[stage] + (threadIdx.x & 15u) * pitch);
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
             for (int b = 0; b < 4; ++b) s[a][b] = 0.0f;
-        for (uint32_t i = 0; i < d; ++i) {
-            const float q0 = q[row * d + i], q1 = q[(row + 1) * d + i];
+#pragma unroll 2
+        for (uint32_t i = 0; i < (d + 3) / 4; ++i) {
+            const float4 u = q0[i], v = q1[i];
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                const float x = k[(key + 16u * b) * (d + 1) + i];
-                s[0][b] = fmaf(q0, x, s[0][b]);
-                s[1][b] = fmaf(q1, x, s[1][b]);
+                const float4 y = x[b * 16 * (pitch / 4) + i];
+                s[0][b] = fmaf(u.x, y.x, fmaf(u.y, y.y, fmaf(u.z, y.z, fmaf(u.w, y.w, s[0][b]))));
+                s[1][b] = fmaf(v.x, y.x, fmaf(v.y, y.y, fmaf(v.z, y.z, fmaf(v.w, y.w, s[1][b]))));
             }
         }
     }
 };
 
-__global__ __launch_bounds__(128) void weigh_stats_any_kernel(const WeighParams p) {
+__global__ __launch_bounds__(kAnyThreads) void weigh_stats_any_kernel(const WeighParams p) {
     extern __shared__ __align__(16) float any_smem[];
     __shared__ uint32_t last_arrival;
     await_previous_kernel();
@@ -377,11 +422,11 @@ __global__ __launch_bounds__(128) void weigh_stats_any_kernel(const WeighParams 
     const uint32_t total = reqs[count].cu0;
     const PageBounds bounds(p.geo);
     uint32_t bad = 0;
-    AnyTile tile(any_smem, p.geo.head_dim);
+    AnyTile tile(any_smem, p);
     const uint32_t at = 2u * (threadIdx.x >> 4), column = threadIdx.x & 15u;
     for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
         const WeighRequest rq = reqs[find_request<0>(reqs, count, item)];
-        const uint32_t pieces = weigh_pieces(rq.keys), rows = rq.q_len * p.group, blocks = (rows + kAnyRows - 1) / kAnyRows;
+        const uint32_t pieces = weigh_pieces(rq.keys, false), rows = rq.q_len * p.group, blocks = (rows + kAnyRows - 1) / kAnyRows;
         const uint32_t local = item - rq.cu0, piece = local % pieces, unit = local / pieces;
         const uint32_t head = unit / blocks, row0 = (unit % blocks) * kAnyRows;
         const uint32_t piece_keys = weigh_piece_keys(rq.keys, pieces);
@@ -389,12 +434,21 @@ __global__ __launch_bounds__(128) void weigh_stats_any_kernel(const WeighParams 
         const uint32_t k1 = min(min(k0 + piece_keys, rq.keys), row_limit(p, rq, min(row0 + kAnyRows, rows) - 1));
         const uint32_t* row_ids = table_row(p.geo, rq.slot);
         Stat st[2] = {{-kInf, 0.0f}, {-kInf, 0.0f}};
-        tile.load_rows(p, rq, head, row0, rows);
-        for (uint32_t key0 = k0; key0 < k1; key0 += kBlock) {
-            tile.load_keys(p, bounds, row_ids, head, key0, k1, bad);
+        uint32_t stage = 0;
+        if (k0 < k1) {
+            tile.load_rows(tile.q, p, rq, head, row0, rows);
+            tile.load_keys(0, p, bounds, row_ids, head, k0, k1, bad);
+        }
+        for (uint32_t key0 = k0; key0 < k1; key0 += kBlock, stage ^= 1u) {
+            if (key0 + kBlock < k1) {
+                tile.load_keys(stage ^ 1u, p, bounds, row_ids, head, key0 + kBlock, k1, bad);
+                cp_async_wait<1>();
+            } else {
+                cp_async_wait<0>();
+            }
             __syncthreads();
             float s[2][4];
-            tile.product(s);
+            tile.product(tile.q, stage, s);
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
                 const uint32_t row = row0 + at + a, limit = row < rows ? min(k1, row_limit(p, rq, row)) : 0u;
@@ -453,10 +507,11 @@ __global__ __launch_bounds__(128) void weigh_stats_any_kernel(const WeighParams 
     if (bad != 0) record_page_fault(p.geo);
 }
 
-__global__ __launch_bounds__(128) void weigh_sum_any_kernel(const WeighParams p) {
+__global__ __launch_bounds__(kAnyThreads) void weigh_sum_any_kernel(const WeighParams p) {
     extern __shared__ __align__(16) float any_smem[];
-    __shared__ float sums[8][kBlock];
-    __shared__ float2 norms[kAnyRows];
+    __shared__ float sums[kAnyRows / 2][kBlock];
+    __shared__ float2 norms[2][kAnyRows];
+    __shared__ uint32_t last_arrival;
     await_previous_kernel();
     const uint32_t count = p.scalars[kScalarWeighLong];
     if (count == 0) return;
@@ -464,38 +519,75 @@ __global__ __launch_bounds__(128) void weigh_sum_any_kernel(const WeighParams p)
     const uint32_t total = reqs[count].cu1;
     const PageBounds bounds(p.geo);
     uint32_t bad = 0;
-    AnyTile tile(any_smem, p.geo.head_dim);
+    AnyTile tile(any_smem, p);
+    float* const row_buffers[2] = {tile.q, tile.k[1]};  // the keys stay: the second key block's place holds the next rows
     const uint32_t at = 2u * (threadIdx.x >> 4), column = threadIdx.x & 15u;
     for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
         const WeighRequest rq = reqs[find_request<1>(reqs, count, item)];
-        const uint32_t rows = rq.q_len * p.group, key_blocks = (rq.keys + kBlock - 1) / kBlock;
-        const uint32_t head = (item - rq.cu1) / key_blocks, key0 = (item - rq.cu1) % key_blocks * kBlock;
-        const uint32_t row_begin = key0 > rq.first_pos ? (key0 - rq.first_pos) * p.group : 0u;
+        const uint32_t all_rows = rq.q_len * p.group, spans = weigh_spans(rq.keys, false);
+        const uint32_t parts = p.split_rows != 0 ? weigh_row_parts(all_rows, rq.keys, p.geo.num_kv_heads, false) : 1u;
+        const uint32_t local = item - rq.cu1, part = local % parts, unit = local / parts;
+        const uint32_t head = unit / spans, key0 = unit % spans * kBlock, each = weigh_part_blocks(all_rows, parts, false) * kAnyRows;
+        const uint32_t rows = min((part + 1) * each, all_rows);
+        const uint32_t seen_from = key0 > rq.first_pos ? (key0 - rq.first_pos) * p.group : 0u;  // rows before see none of the keys
+        const uint32_t row_begin = max(part * each, seen_from);
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        tile.load_keys(p, bounds, table_row(p.geo, rq.slot), head, key0, rq.keys, bad);
-        for (uint32_t row0 = row_begin; row0 < rows; row0 += kAnyRows) {
-            tile.load_rows(p, rq, head, row0, rows);
-            if (threadIdx.x < kAnyRows) norms[threadIdx.x] = row0 + threadIdx.x < rows ? p.norms[query_row(p, rq, head, row0 + threadIdx.x)] : make_float2(kInf, 0.0f);
+        const auto fetch = [&](uint32_t row0, uint32_t stage) {
+            tile.load_rows(row_buffers[stage], p, rq, head, row0, all_rows);
+            if (threadIdx.x < kAnyRows)
+                norms[stage][threadIdx.x] = row0 + threadIdx.x < rows ? p.norms[query_row(p, rq, head, row0 + threadIdx.x)] : make_float2(kInf, 0.0f);
+            cp_async_commit();
+        };
+        tile.load_keys(0, p, bounds, table_row(p.geo, rq.slot), head, key0, rq.keys, bad);
+        if (row_begin < rows) fetch(row_begin, 0);
+        uint32_t stage = 0;
+        for (uint32_t row0 = row_begin; row0 < rows; row0 += kAnyRows, stage ^= 1u) {
+            if (row0 + kAnyRows < rows) {
+                fetch(row0 + kAnyRows, stage ^ 1u);
+                cp_async_wait<1>();
+            } else {
+                cp_async_wait<0>();
+            }
             __syncthreads();
             float s[2][4];
-            tile.product(s);
+            tile.product(row_buffers[stage], 0, s);
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
                 const uint32_t row = row0 + at + a, limit = row < rows ? row_limit(p, rq, row) : 0u;
 #pragma unroll
                 for (int b = 0; b < 4; ++b)
-                    if (key0 + column + 16u * b < limit) sum[b] += weight_of(s[a][b], p.scale_log2, norms[at + a]);
+                    if (key0 + column + 16u * b < limit) sum[b] += weight_of(s[a][b], p.scale_log2, norms[stage][at + a]);
             }
             __syncthreads();
         }
+        cp_async_wait<0>();
 #pragma unroll
         for (int b = 0; b < 4; ++b) sums[threadIdx.x >> 4][column + 16u * b] = sum[b];
         __syncthreads();
-        if (threadIdx.x < kBlock && key0 + threadIdx.x < rq.keys) {
-            float all = 0.0f;
+        float all = 0.0f;
+        if (threadIdx.x < kBlock) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) all += sums[i][threadIdx.x];
-            weight_row(p, rq, head)[key0 + threadIdx.x] += all;
+            for (uint32_t i = 0; i < kAnyRows / 2; ++i) all += sums[i][threadIdx.x];
+        }
+        const bool mine = threadIdx.x < kBlock && key0 + threadIdx.x < rq.keys;
+        if (parts == 1) {
+            if (mine) weight_row(p, rq, head)[key0 + threadIdx.x] += all;
+        } else {  // the last part of the span adds up the parts
+            if (mine) p.sums[uint64_t(item) * kBlock + threadIdx.x] = all;
+            __threadfence();
+            __syncthreads();
+            uint32_t* counter = p.long_counters() + rq.cu1 + unit * parts;
+            if (threadIdx.x == 0) last_arrival = atomicAdd(counter, 1u) == parts - 1 ? 1u : 0u;
+            __syncthreads();
+            if (last_arrival != 0) {
+                __threadfence();
+                if (mine) {
+                    float whole = 0.0f;
+                    for (uint32_t o = 0; o < parts; ++o) whole += __ldcg(p.sums + uint64_t(rq.cu1 + unit * parts + o) * kBlock + threadIdx.x);
+                    weight_row(p, rq, head)[key0 + threadIdx.x] += whole;
+                }
+                if (threadIdx.x == 0) *counter = 0;
+            }
         }
         __syncthreads();
     }
@@ -532,14 +624,14 @@ cudaError_t launch_typed(const WeighParams& p, WeighPass pass, uint32_t ctas, cu
 }
 
 cudaError_t launch_any(const WeighParams& p, WeighPass pass, uint32_t ctas, cudaStream_t stream) {
-    const int most = int((kAnyRows * 256 + kBlock * 257) * sizeof(float));
-    const size_t smem = (kAnyRows * p.geo.head_dim + kBlock * (p.geo.head_dim + 1)) * sizeof(float);
+    const int most = int((kAnyRows + 2 * kBlock) * any_pitch(256) * sizeof(float));
+    const size_t smem = (kAnyRows + 2 * kBlock) * any_pitch(p.geo.head_dim) * sizeof(float);
     static std::atomic<uint64_t> stats_done{0}, sum_done{0};
     const bool stats = pass == WeighPass::kLongStats;
     const cudaError_t err = stats ? ensure_dynamic_smem(reinterpret_cast<const void*>(weigh_stats_any_kernel), most, stats_done)
                                   : ensure_dynamic_smem(reinterpret_cast<const void*>(weigh_sum_any_kernel), most, sum_done);
     if (err != cudaSuccess) return err;
-    return launch_overlapped(stats ? weigh_stats_any_kernel : weigh_sum_any_kernel, dim3(ctas), dim3(128), smem, stream, p);
+    return launch_overlapped(stats ? weigh_stats_any_kernel : weigh_sum_any_kernel, dim3(ctas), dim3(kAnyThreads), smem, stream, p);
 }
 
 }  // namespace

@@ -11,12 +11,12 @@ namespace psi {
 
 constexpr uint32_t kWeighBlock = 128;    // rows or keys of one block of the long-run kernels
 constexpr uint32_t kWeighSpan = 4;       // key blocks of one second-pass item of theirs
-constexpr uint32_t kWeighAnyRows = 16;   // rows and keys of one block of the CUDA-core kernels
+constexpr uint32_t kWeighAnyRows = 32;   // rows and keys of one block of the CUDA-core kernels
 constexpr uint32_t kWeighAnyKeys = 64;
 constexpr uint32_t kWeighShortRows = 16; // query rows of a KV head up to which a run goes to the short-run kernel
 constexpr uint32_t kWeighTile = 32;      // keys of one unit of the short-run kernel's shares
-constexpr uint32_t kWeighPieceKeys = 1024;
-constexpr uint32_t kWeighMaxPieces = 16;
+constexpr uint32_t kWeighPieceKeys = 1024, kWeighMaxPieces = 16;       // of the first pass on the tensor cores
+constexpr uint32_t kWeighAnyPieceKeys = 256, kWeighAnyMaxPieces = 64;  // and on the CUDA cores
 
 // A request with tokens as the kernels see it.  Short runs first, then one entry that ends their prefix sums, then the long
 // runs and one entry that ends theirs.
@@ -29,10 +29,11 @@ struct WeighRequest {
 };
 constexpr uint64_t kWeighRequestWords = sizeof(WeighRequest) / sizeof(uint32_t);
 
-// A long run's keys are cut into pieces of 1,024 or more, at most sixteen, so that the scratch does not grow with the context.
-__host__ __device__ inline uint32_t weigh_pieces(uint32_t keys) {
-    const uint32_t n = keys / kWeighPieceKeys + (keys % kWeighPieceKeys != 0 ? 1u : 0u);
-    return n < kWeighMaxPieces ? n : kWeighMaxPieces;
+// A long run's keys are cut into a bounded number of pieces, so that the scratch does not grow with the context.
+__host__ __device__ inline uint32_t weigh_pieces(uint32_t keys, bool tensor) {
+    const uint32_t each = tensor ? kWeighPieceKeys : kWeighAnyPieceKeys, most = tensor ? kWeighMaxPieces : kWeighAnyMaxPieces;
+    const uint32_t n = keys / each + (keys % each != 0 ? 1u : 0u);
+    return n < most ? n : most;
 }
 // Keys of one piece, in whole blocks.
 __host__ __device__ inline uint32_t weigh_piece_keys(uint32_t keys, uint32_t pieces) {
@@ -40,10 +41,24 @@ __host__ __device__ inline uint32_t weigh_piece_keys(uint32_t keys, uint32_t pie
     return (each + kWeighBlock - 1) / kWeighBlock * kWeighBlock;  // (a multiple of kWeighAnyKeys as well)
 }
 
-// Second-pass items of one KV head: spans of key blocks on the tensor cores, blocks of 64 keys on the CUDA cores.
-inline uint64_t weigh_sum_items(uint32_t keys, bool tensor) {
-    const uint64_t each = tensor ? kWeighBlock * kWeighSpan : kWeighAnyKeys;
-    return (keys + each - 1) / each;
+// Second-pass spans of one KV head: blocks of keys on the tensor cores, 64 keys on the CUDA cores.
+__host__ __device__ constexpr uint32_t weigh_span_keys(bool tensor) { return tensor ? kWeighBlock * kWeighSpan : kWeighAnyKeys; }
+__host__ __device__ inline uint32_t weigh_spans(uint32_t keys, bool tensor) {
+    return keys / weigh_span_keys(tensor) + (keys % weigh_span_keys(tensor) != 0 ? 1u : 0u);
+}
+// Into how many parts a run's rows are cut in the second pass, each an item of its own whose sums the last one adds up: where the spans
+// of all KV heads are fewer than two for each SM of a B200, and a part has two row blocks left.
+__host__ __device__ inline uint32_t weigh_row_parts(uint32_t rows, uint32_t keys, uint32_t heads, bool tensor) {
+    const uint64_t spans = uint64_t(weigh_spans(keys, tensor)) * heads;
+    if (spans >= 296) return 1;
+    const uint32_t least = tensor ? 2 * kWeighBlock : 2 * kWeighAnyRows;
+    const uint32_t wanted = uint32_t((296 + spans - 1) / spans), most = rows / least > 0 ? rows / least : 1;
+    return wanted < most ? wanted : most;
+}
+// Row blocks of one part.
+__host__ __device__ inline uint32_t weigh_part_blocks(uint32_t rows, uint32_t parts, bool tensor) {
+    const uint32_t block = tensor ? kWeighBlock : kWeighAnyRows, blocks = (rows + block - 1) / block;
+    return (blocks + parts - 1) / parts;
 }
 
 inline bool weigh_on_tensor_cores(uint32_t dtype, uint32_t head_dim) { return dtype != PSI_DTYPE_F32 && head_dim % 8 == 0; }
@@ -61,6 +76,8 @@ struct WeighParams {
     uint64_t long_partials_at;
     uint32_t* counters;           // arrivals by unit, zero between launches: short runs, then long ones
     uint64_t long_counters_at;
+    float* sums;                  // second pass of long runs: [item][keys of a span], where rows are cut into parts
+    uint32_t split_rows;          // they may be (not in captured launches, whose scratch does not follow the batch)
     float* scores;                // short runs: [tiles][4][score_rows][8]
     uint32_t score_rows;          // most query rows of a short run
     uint32_t group;               // q heads of a KV head

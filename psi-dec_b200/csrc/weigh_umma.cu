@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks <= 2 ? 2 : 1) weigh_umma_ker
         const uint32_t* row_ids = table_row(p.geo, rq.slot);
         uint32_t head, block_begin, block_end, k_begin, k_end, pieces = 1, unit = 0;
         if (kStats) {
-            pieces = weigh_pieces(rq.keys);
+            pieces = weigh_pieces(rq.keys, true);
             const uint32_t local = item - rq.cu0, piece = local % pieces, piece_keys = weigh_piece_keys(rq.keys, pieces);
             unit = local / pieces;
             head = unit / blocks;
@@ -123,15 +123,22 @@ __global__ void __launch_bounds__(kThreads, kBlocks <= 2 ? 2 : 1) weigh_umma_ker
             k_begin = piece * piece_keys;
             k_end = min(k_begin + piece_keys, rq.keys);
         } else {
-            const uint32_t spans = (rq.keys + kRows * kWeighSpan - 1) / (kRows * kWeighSpan), local = item - rq.cu1;
-            head = local / spans;
-            block_begin = 0;
-            block_end = blocks;
-            k_begin = local % spans * (kRows * kWeighSpan);
-            k_end = min(k_begin + kRows * kWeighSpan, rq.keys);
+            pieces = p.split_rows != 0 ? weigh_row_parts(rows, rq.keys, p.geo.num_kv_heads, true) : 1u;
+            const uint32_t spans = weigh_spans(rq.keys, true), local = item - rq.cu1, part = local % pieces, each = weigh_part_blocks(rows, pieces, true);
+            unit = local / pieces;
+            head = unit / spans;
+            block_begin = part * each;
+            block_end = min(block_begin + each, blocks);
+            k_begin = unit % spans * weigh_span_keys(true);
+            k_end = min(k_begin + weigh_span_keys(true), rq.keys);
             // rows of tokens before the span's first key see none of it
-            if (k_begin > rq.first_pos) block_begin = (k_begin - rq.first_pos) * p.group / kRows;
+            if (k_begin > rq.first_pos) block_begin = max(block_begin, uint32_t(uint64_t(k_begin - rq.first_pos) * p.group / kRows));
+            if (pieces > 1)
+                for (uint32_t i = tid; i < weigh_span_keys(true); i += kThreads) p.sums[uint64_t(item) * weigh_span_keys(true) + i] = 0.0f;
+            __syncthreads();
         }
+        // where a key's sum goes: its weight, or this part's share of it
+        float* const sums = kStats ? nullptr : pieces > 1 ? p.sums + uint64_t(item) * weigh_span_keys(true) - k_begin : weight_row(p, rq, head);
         for (uint32_t block = block_begin; block < block_end; ++block) {
             const uint32_t row0 = block * kRows;
             const uint32_t seen = min(k_end, row_limit(p, rq, min(row0 + kRows, rows) - 1));  // keys that a row of the block sees end here
@@ -232,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks <= 2 ? 2 : 1) weigh_umma_ker
                     const float2 all = unpack_f32x2(add_f32x2(sum[0], sum[1]));
                     if (half == 1) sh.half[row].x = all.x + all.y;
                     asm volatile("bar.sync %0, 64;" ::"r"((warp & 3u) + 1) : "memory");  // the warps of these lanes
-                    if (half == 0 && key < k_end) weight_row(p, rq, head)[key] += all.x + all.y + sh.half[row].x;
+                    if (half == 0 && key < k_end) sums[key] += all.x + all.y + sh.half[row].x;
                 }
             };
             for (uint32_t tile = 0; tile < tiles; ++tile) {
@@ -300,6 +307,25 @@ __global__ void __launch_bounds__(kThreads, kBlocks <= 2 ? 2 : 1) weigh_umma_ker
                     }
                     __syncthreads();
                 }
+            }
+        }
+        if constexpr (!kStats) {
+            if (pieces > 1) {  // the last part of the span adds up the parts
+                __threadfence();
+                __syncthreads();
+                uint32_t* counter = p.long_counters() + rq.cu1 + unit * pieces;
+                if (tid == 0) sh.last_arrival = atomicAdd(counter, 1u) == pieces - 1 ? 1u : 0u;
+                __syncthreads();
+                if (sh.last_arrival != 0) {
+                    __threadfence();
+                    for (uint32_t i = tid; i < k_end - k_begin; i += kThreads) {
+                        float all = 0.0f;
+                        for (uint32_t o = 0; o < pieces; ++o) all += __ldcg(p.sums + uint64_t(rq.cu1 + unit * pieces + o) * weigh_span_keys(true) + i);
+                        weight_row(p, rq, head)[k_begin + i] += all;
+                    }
+                    if (tid == 0) *counter = 0;
+                }
+                __syncthreads();
             }
         }
     }
