@@ -9,6 +9,7 @@
 #include "device_common.cuh"
 #include "launch_util.hpp"
 #include "linear_attend.hpp"
+#include "umma_common.cuh"
 
 namespace psi {
 
@@ -21,7 +22,7 @@ constexpr uint32_t kStepTokens = 8;                         // tokens whose rows
 
 template <int kRows>  // of the state in one thread: key_dim <= 16 kRows
 __global__ __launch_bounds__(kStepThreads) void linear_step_kernel(const LinearParams p) {
-    __shared__ float q_rows[kStepTokens][kRows * 16], k_rows[kStepTokens][kRows * 16];
+    __shared__ float2 rows[kStepTokens][kRows * 16];  // (k, q)
     __shared__ __align__(16) float v_cols[kStepTokens][kStepColumns];
     __shared__ __align__(16) float sums[kStepTokens][kStepThreads / 32][kStepColumns];
     await_previous_kernel();
@@ -35,22 +36,22 @@ __global__ __launch_bounds__(kStepThreads) void linear_step_kernel(const LinearP
         const uint32_t col = slice * kStepColumns + 4u * quad;
         const bool live = col < p.value_dim;  // value_dim is a multiple of eight
         const float* from = p.state_of(rq.src, head);
-        float4 s[kRows];
+        ulonglong2 s[kRows];  // four columns, two in each word
 #pragma unroll
         for (int j = 0; j < kRows; ++j) {
             const uint32_t row = group + kStepRowGroups * j;
-            s[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (rq.fresh == 0 && live && row < p.key_dim) s[j] = *reinterpret_cast<const float4*>(from + uint64_t(row) * p.value_dim + col);
+            s[j] = make_ulonglong2(0, 0);
+            if (rq.fresh == 0 && live && row < p.key_dim) s[j] = *reinterpret_cast<const ulonglong2*>(from + uint64_t(row) * p.value_dim + col);
         }
         const float hi = p.decays[head * kLinearDecays + 1], lo = p.decays[head * kLinearDecays + kLinearStepLow];
+        const uint64_t hi2 = pack_f32x2(hi, hi), lo2 = pack_f32x2(lo, lo);
         for (uint32_t t0 = 0; t0 < rq.q_len; t0 += kStepTokens) {
             const uint32_t tokens = min(kStepTokens, rq.q_len - t0);
             __syncthreads();
             for (uint32_t i = threadIdx.x; i < tokens * kRows * 16u; i += kStepThreads) {
                 const uint32_t t = i / (kRows * 16u), d = i % (kRows * 16u);
                 const uint64_t at = (uint64_t(rq.flat_begin + t0 + t) * p.num_k_heads + head / share) * p.key_dim + d;
-                q_rows[t][d] = d < p.key_dim ? load_as_float(p.q, at, p.dtype) : 0.0f;
-                k_rows[t][d] = d < p.key_dim ? load_as_float(p.k, at, p.dtype) : 0.0f;
+                rows[t][d] = d < p.key_dim ? make_float2(load_as_float(p.k, at, p.dtype), load_as_float(p.q, at, p.dtype)) : make_float2(0.0f, 0.0f);
             }
             for (uint32_t i = threadIdx.x; i < tokens * kStepColumns; i += kStepThreads) {
                 const uint32_t t = i / kStepColumns, c = slice * kStepColumns + i % kStepColumns;
@@ -59,20 +60,19 @@ __global__ __launch_bounds__(kStepThreads) void linear_step_kernel(const LinearP
             }
             __syncthreads();
             for (uint32_t t = 0; t < tokens; ++t) {
-                const float4 v = *reinterpret_cast<const float4*>(&v_cols[t][4u * quad]);
-                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&v_cols[t][4u * quad]);
+                uint64_t o_xy = 0, o_zw = 0;
 #pragma unroll
                 for (int j = 0; j < kRows; ++j) {
-                    const float k = k_rows[t][group + kStepRowGroups * j], q = q_rows[t][group + kStepRowGroups * j];
-                    s[j].x = fmaf(hi, s[j].x, fmaf(lo, s[j].x, k * v.x));
-                    s[j].y = fmaf(hi, s[j].y, fmaf(lo, s[j].y, k * v.y));
-                    s[j].z = fmaf(hi, s[j].z, fmaf(lo, s[j].z, k * v.z));
-                    s[j].w = fmaf(hi, s[j].w, fmaf(lo, s[j].w, k * v.w));
-                    o.x = fmaf(q, s[j].x, o.x);
-                    o.y = fmaf(q, s[j].y, o.y);
-                    o.z = fmaf(q, s[j].z, o.z);
-                    o.w = fmaf(q, s[j].w, o.w);
+                    const float2 kq = rows[t][group + kStepRowGroups * j];
+                    const uint64_t k = pack_f32x2(kq.x, kq.x), q = pack_f32x2(kq.y, kq.y);
+                    s[j].x = fma_f32x2(hi2, s[j].x, fma_f32x2(lo2, s[j].x, mul_f32x2(k, v.x)));
+                    s[j].y = fma_f32x2(hi2, s[j].y, fma_f32x2(lo2, s[j].y, mul_f32x2(k, v.y)));
+                    o_xy = fma_f32x2(q, s[j].x, o_xy);
+                    o_zw = fma_f32x2(q, s[j].y, o_zw);
                 }
+                const float2 xy = unpack_f32x2(o_xy), zw = unpack_f32x2(o_zw);
+                float4 o = make_float4(xy.x, xy.y, zw.x, zw.y);
 #pragma unroll
                 for (int x = 8; x < 32; x <<= 1) {
                     o.x += __shfl_xor_sync(0xFFFFFFFFu, o.x, x);
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(kStepThreads) void linear_step_kernel(const LinearP
 #pragma unroll
         for (int j = 0; j < kRows; ++j) {
             const uint32_t row = group + kStepRowGroups * j;
-            if (live && row < p.key_dim) *reinterpret_cast<float4*>(to + uint64_t(row) * p.value_dim + col) = s[j];
+            if (live && row < p.key_dim) *reinterpret_cast<ulonglong2*>(to + uint64_t(row) * p.value_dim + col) = s[j];
         }
     }
 }
