@@ -5,9 +5,11 @@
 // inside a thread, and what belongs to a row (its maximum, 1 / sum and limit) is read from shared memory.  The query rows
 // of an item stay in shared memory, key blocks pass by in a ring of two (cp.async from their pages, any page size), and the MMA of
 // a block runs under the exponentials of the block before: two S buffers in TMEM.  Threads w and w + 128 share a lane, half of the
-// columns each.  Bound by the special-function unit: 128 x 128 exponentials take 1,024 cycles a tile and pass, its product 512 (at
-// head_dim 128).  A quarter of the exponentials is therefore worked out on the FMA pipe (exp2_fma).  Two CTAs share an SM at head_dim
-// 128 and below, so that one's loads and barriers run under the other's arithmetic.
+// columns each.  Bound by issue slots: a tile's 128 x 128 exponentials take 1,024 cycles of the special-function unit in each pass and
+// its product 512 of the tensor pipe (at head_dim 128), but an element takes about four instructions beside its exponential.  (A
+// quarter of the exponentials as polynomials on the FMA pipe cost more slots than they freed: 68 and 80 us for the passes over
+// four prompts of 4,099 to 16,384 keys, 64 tokens of 32/8 heads x 128 each.)  Two CTAs share an SM at head_dim 128 and below, so that
+// one's loads and barriers run under the other's arithmetic.
 // Every mbarrier wait is bounded and reports PSI_ERR_TIMEOUT through the status word, and TMEM is freed on every path.
 #include "launch_util.hpp"
 #include "umma_common.cuh"
@@ -31,32 +33,11 @@ struct UmmaWeighShared {
     uint64_t offsets[2][kRows];           // element offsets of the rows of a ring slot's next block
 };
 
-// 2^x on the FMA pipe for -126 <= x <= 0 (0 below): x = n + f with n whole and f in [-1/2, 1/2], 2^f as the Taylor polynomial of
-// e^(f ln 2) to the seventh power, whose next term is at most (ln 2 / 2)^8 / 8! = 5e-9.
-__device__ __forceinline__ float exp2_fma(float x) {
-    const float clamped = fmaxf(x, -126.0f);
-    const float shifted = clamped + 12582912.0f;  // 1.5 * 2^23: the sum's last bits hold n
-    const float f = clamped - (shifted - 12582912.0f);
-    float y = 1.5252734e-5f;        // ln(2)^7 / 7!
-    y = fmaf(y, f, 1.5403530e-4f);  // ln(2)^6 / 6!
-    y = fmaf(y, f, 1.3333558e-3f);
-    y = fmaf(y, f, 9.6181291e-3f);
-    y = fmaf(y, f, 5.5504109e-2f);
-    y = fmaf(y, f, 2.4022651e-1f);
-    y = fmaf(y, f, 6.9314718e-1f);
-    y = fmaf(y, f, 1.0f);
-    const float scaled = __int_as_float(__float_as_int(y) + (__float_as_int(shifted) << 23));
-    return x < -126.0f ? 0.0f : scaled;
-}
-
-// Every fourth exponential goes to the FMA pipe.
-__device__ __forceinline__ float exp2_mixed(float x, int index) { return index % 4 == 3 ? exp2_fma(x) : exp2_approx(x); }
-
 // kBlocks: 64-element blocks of a row.  kStats: first pass.
 template <typename T, uint32_t kBlocks, bool kStats>
 __global__ void __launch_bounds__(kThreads, kBlocks <= 2 ? 2 : 1) weigh_umma_kernel(const WeighParams p) {
     constexpr uint32_t kTileBytes = kBlocks * kRows * 128;  // a block of 128 rows: [64-element block][row][128 bytes, swizzled]
-    constexpr uint32_t kChunks = kBlocks * 8;
+    constexpr uint32_t kLanes = kBlocks == 3 ? 32 : kBlocks * 8;  // threads that copy a row, a chunk each
     __shared__ UmmaWeighShared sh;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const uint32_t tid = threadIdx.x, warp = tid >> 5;
@@ -96,14 +77,19 @@ __global__ void __launch_bounds__(kThreads, kBlocks <= 2 ? 2 : 1) weigh_umma_ker
             if (p.geo.fault != nullptr) atomicExch(p.geo.fault, uint32_t(PSI_ERR_TIMEOUT));
         }
     };
-    // Copies 128 rows whose element offsets stand in shared memory (~0: zeros) into a block; a row's chunks lie in neighbouring lanes.
+    // Copies 128 rows whose element offsets stand in shared memory (~0: zeros) into a block.  A thread's chunk and its place in the
+    // swizzle stay the same from row to row: its rows are a multiple of eight apart.
+    const uint32_t copy_row = tid / kLanes, copy_chunk = tid % kLanes;
+    const uint32_t copy_at = (copy_chunk >> 3) * (kRows * 128) + copy_row * 128 + (((copy_chunk ^ copy_row) & 7u) << 4);
+    const bool copies = copy_chunk < kBlocks * 8, has_data = copy_chunk < chunks;
     const auto copy_block = [&](uint32_t dst, const void* base, const uint64_t* offsets) {
-        for (uint32_t at = tid; at < kRows * kChunks; at += kThreads) {
-            const uint32_t r = at / kChunks, c = at % kChunks;
-            const uint64_t offset = offsets[r];
-            const bool live = offset != ~0ull && c < chunks;
-            cp_async_16(dst + (c >> 3) * (kRows * 128) + r * 128 + (((c ^ r) & 7u) << 4),
-                        static_cast<const uint16_t*>(base) + (live ? offset + c * 8u : 0u), live ? 16u : 0u);
+        if (!copies) return;
+        const uint16_t* from = static_cast<const uint16_t*>(base) + (has_data ? copy_chunk * 8u : 0u);
+#pragma unroll
+        for (uint32_t r = 0; r < kRows; r += kThreads / kLanes) {
+            const uint64_t offset = offsets[copy_row + r];
+            const bool live = has_data && offset != ~0ull;
+            cp_async_16(dst + copy_at + r * 128, from + (live ? offset : 0u), live ? 16u : 0u);
         }
     };
 
@@ -202,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks <= 2 ? 2 : 1) weigh_umma_ker
 #pragma unroll
                     for (int c = 0; c < 64; c += 2) {
                         const float2 x = unpack_f32x2(fma_f32x2(pack_f32x2(s[c], s[c + 1]), scale2, base2));
-                        sum[(c >> 1) & 1] = add_f32x2(sum[(c >> 1) & 1], pack_f32x2(exp2_mixed(x.x, c), exp2_mixed(x.y, c + 1)));
+                        sum[(c >> 1) & 1] = add_f32x2(sum[(c >> 1) & 1], pack_f32x2(exp2_approx(x.x), exp2_approx(x.y)));
                     }
                     const float2 all = unpack_f32x2(add_f32x2(sum[0], sum[1]));
                     st.l += all.x + all.y;
@@ -223,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks <= 2 ? 2 : 1) weigh_umma_ker
                             float2 x = unpack_f32x2(fma_f32x2(pack_f32x2(s[c], s[c + 1]), scale2, base.x));
                             float2 y = unpack_f32x2(fma_f32x2(pack_f32x2(s[c + 2], s[c + 3]), scale2, base.y));
                             x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-                            y = make_float2(exp2_approx(y.x), exp2_mixed(y.y, 3));
+                            y = make_float2(exp2_approx(y.x), exp2_approx(y.y));
                             if (masked) {
                                 const uint4 limit = *reinterpret_cast<const uint4*>(&sh.limit[column0 + c0 + c]);
                                 const float2 i0 = unpack_f32x2(inverse.x), i1 = unpack_f32x2(inverse.y);
