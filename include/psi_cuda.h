@@ -644,7 +644,9 @@ PSI_API int32_t psi_linear_set_decay(psi_linear* linear, uint32_t layer, const f
 PSI_API int32_t psi_linear_prepare(psi_linear* linear, const uint32_t* req_slots, const uint32_t* out_slots,
                                    const uint32_t* token_indices, const uint32_t* cu_tokens, uint32_t num_reqs);
 /* q, k device [T][Hk][key_dim], v, out device [T][Hv][value_dim]; out must not overlap the inputs.  Any number of tokens per
- * request.  The same call gives the same bits.  May be captured: a replay takes the batch prepared last. */
+ * request.  The same call gives the same bits.  May be captured: a replay takes the batch prepared last, and the buffers of a
+ * captured call hold max_tokens rows, whatever batch comes (rows behind the batch are read over and not used).  A token whose
+ * q, k or v is not finite reaches no token before it and no other request. */
 PSI_API int32_t psi_linear_attend(psi_linear* linear, uint32_t layer, float* states, const void* q, const void* k, const void* v,
                                   void* out);
 /* As psi_gqa_device_status: waits for the stream; PSI_ERR_TIMEOUT when a bounded wait of a launch gave up. */

@@ -28,6 +28,7 @@ using GQAPageTableLayout = psi_page_table_layout;
 using GQAReplayShape = psi_replay_shape;
 using GQASplitKVVariant = psi_split_kv_variant;
 using GQAConfig = psi_gqa_config;
+using LinearConfig = psi_linear_config;
 using NormRopeConfig = psi_norm_rope_config;
 
 // A call that did not return PSI_OK.  The reference panics where this is thrown for PSI_ERR_INVALID_ARGUMENT.
@@ -373,6 +374,25 @@ public:
                                         cu_tokens.data(), static_cast<uint32_t>(req_slots.size()), k_host, v_host, q_host,
                                         out_host), ctx_);
     }
+    // Adds the attention weight that the prepared batch's queries give each cached key to weights, device f32
+    // [num_req_slots][Hkv][weights_stride].
+    void weigh_keys(PageArena& pages, GQARequestPageTable& table, uint32_t layer, const void* q, float* weights,
+                    uint64_t weights_stride) {
+        detail::check(psi_gqa_weigh_keys(handle(), pages.handle(), table.handle(), layer, q, weights, weights_stride), ctx_);
+    }
+    // Cuts caches down to their last `recent` and heaviest keys, in place or into another slot; kept is device u32
+    // [requests][Hkv][kept_stride].
+    void evict(PageArena& pages, GQARequestPageTable& table, uint32_t layer, const std::vector<uint32_t>& src_slots,
+               const std::vector<uint32_t>& dst_slots, const std::vector<uint32_t>& lengths, const std::vector<uint32_t>& keeps,
+               uint32_t recent, const float* weights, float* weights_out, uint64_t weights_stride, uint32_t* kept,
+               uint64_t kept_stride) {
+        if (dst_slots.size() != src_slots.size() || lengths.size() != src_slots.size() || keeps.size() != src_slots.size()) {
+            throw Error(PSI_ERR_INVALID_ARGUMENT, "src_slots, dst_slots, lengths and keeps lengths disagree");
+        }
+        detail::check(psi_gqa_evict(handle(), pages.handle(), table.handle(), layer, src_slots.data(), dst_slots.data(),
+                                    lengths.data(), keeps.data(), static_cast<uint32_t>(src_slots.size()), recent, weights,
+                                    weights_out, weights_stride, kept, kept_stride), ctx_);
+    }
     // Waits for the stream, then returns and clears what a bounded device-side wait or bounds check recorded (0: nothing).
     int32_t device_status() {
         int32_t out = 0;
@@ -398,6 +418,47 @@ private:
     }
     psi_ctx* ctx_;
     GQAConfig config_;
+    Owner handle_;
+};
+
+// Linear attention with a decay per value head: a state for each request slot instead of a cache.
+class LinearAttention {
+public:
+    LinearAttention(Context& ctx, const LinearConfig& config) : ctx_(ctx.handle()), config_(config) {
+        psi_linear* raw = nullptr;
+        detail::check(psi_linear_create(ctx_, &config, &raw), ctx_);
+        handle_ = Owner(raw);
+    }
+    psi_linear* handle() const noexcept { return handle_.get(); }
+    const LinearConfig& config() const noexcept { return config_; }
+
+    void set_decay(uint32_t layer, const std::vector<float>& log_decay) {
+        if (log_decay.size() != config_.num_v_heads) throw Error(PSI_ERR_INVALID_ARGUMENT, "log_decay must have a value for each v head");
+        detail::check(psi_linear_set_decay(handle(), layer, log_decay.data()), ctx_);
+    }
+    // out_slots empty: every request's state stays in its slot.
+    void prepare(const std::vector<uint32_t>& req_slots, const std::vector<uint32_t>& token_indices,
+                 const std::vector<uint32_t>& cu_tokens, const std::vector<uint32_t>& out_slots = {}) {
+        if (req_slots.size() != token_indices.size() || cu_tokens.size() != req_slots.size() + 1 ||
+            (!out_slots.empty() && out_slots.size() != req_slots.size())) {
+            throw Error(PSI_ERR_INVALID_ARGUMENT, "req_slots, out_slots, token_indices and cu_tokens lengths disagree");
+        }
+        detail::check(psi_linear_prepare(handle(), req_slots.data(), out_slots.empty() ? nullptr : out_slots.data(),
+                                         token_indices.data(), cu_tokens.data(), static_cast<uint32_t>(req_slots.size())), ctx_);
+    }
+    void attend(uint32_t layer, float* states, const void* q, const void* k, const void* v, void* out) {
+        detail::check(psi_linear_attend(handle(), layer, states, q, k, v, out), ctx_);
+    }
+    int32_t device_status() {
+        int32_t out = 0;
+        detail::check(psi_linear_device_status(handle(), &out), ctx_);
+        return out;
+    }
+
+private:
+    using Owner = detail::Handle<psi_linear, psi_linear_destroy>;
+    psi_ctx* ctx_;
+    LinearConfig config_;
     Owner handle_;
 };
 

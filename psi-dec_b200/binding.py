@@ -209,7 +209,8 @@ class Context:
 
     def kernel_timing(self, kernel_class: int):
         """(total milliseconds, launches) of one kernel class (0 append, 1 attend map, 2 attend reduce, 3 combine,
-        4 gather) since timing was enabled."""
+        4 gather, 5 attend chunk, 6 norm + RoPE + append, 7 key weights, 8 eviction, 9 linear attention) since timing was
+        enabled."""
         ms, n = C.c_float(), C.c_uint64()
         _check(library().psi_ctx_kernel_timing(self._h, C.c_uint32(kernel_class), C.byref(ms), C.byref(n)), self._h)
         return ms.value, n.value
