@@ -196,6 +196,12 @@ struct psi_weigh_plan {
     uint32_t short_rows = 0;             // most query rows of a KV head among the short runs
     uint32_t max_keys = 0;
     uint64_t tiles = 0, stats_items = 0, sum_items = 0, long_units = 0;
+    struct LongRun {
+        uint32_t key_blocks;
+        uint64_t units;                  // row blocks times KV heads
+    };
+    std::vector<LongRun> long_runs;      // on the tensor cores
+    uint32_t span_keys = 0;              // of a second-pass item
     bool repeated = false;               // a slot appears twice in the batch
     bool too_large = false;
     bool parted = false;                 // rows of a long run are cut into parts in the second pass

@@ -7,6 +7,57 @@ using namespace psi;
 
 namespace psi {
 
+namespace {
+
+using LongRun = psi_weigh_plan::LongRun;
+
+// Into items of how many key blocks the long runs of a batch are cut, between `least` and kMostBlocks, on the tensor cores.  The CTAs
+// of a wave take items in turn, so that a launch takes as many rounds as items over CTAs, rounded up, of an item each; an item
+// costs kItemStart blocks beside its own (its first loads and product are exposed).  Four prompts' ends of 4,099 to 16,384 keys, 64 tokens of
+// 32/8 heads x 128: pieces of 20 blocks and spans of 9, one round each, 104 us for both passes, against 140 with 8 and 4 (2.3 rounds).
+// Batches of many runs take many rounds of whatever length: theirs is fixed.
+constexpr uint32_t kMostBlocks = 24, kItemStart = 2, kMostRuns = 64;
+
+template <typename Units>
+uint32_t choose_blocks(const psi_gqa* g, const std::vector<LongRun>& runs, uint32_t least, uint32_t otherwise, const Units& units_of) {
+    if (runs.size() > kMostRuns) return std::max(least, otherwise);
+    const uint32_t wave = weigh_wave(g->cfg.head_dim);
+    uint32_t best = least;
+    double least_cost = 1e300;
+    for (uint32_t blocks = least; blocks <= std::max(least, kMostBlocks); ++blocks) {
+        uint64_t items = 0, work = 0;
+        for (const LongRun& run : runs) {
+            const uint64_t cuts = (run.key_blocks + blocks - 1) / blocks;
+            items += units_of(run, false) * cuts;
+            work += units_of(run, true) * (run.key_blocks + cuts * kItemStart);
+        }
+        const double cost = items == 0 ? 0.0 : double((items + wave - 1) / wave) * double(work) / double(items);
+        if (cost < least_cost) {
+            least_cost = cost;
+            best = blocks;
+        }
+    }
+    return best;
+}
+
+// First pass: an item for each unit (row block, KV head) and piece, kWeighMaxPieces pieces at most.
+uint32_t choose_piece(const psi_gqa* g, const std::vector<LongRun>& runs) {
+    uint32_t most = 1;
+    for (const LongRun& run : runs) most = std::max(most, run.key_blocks);
+    const uint32_t least = (most + kWeighMaxPieces - 1) / kWeighMaxPieces;
+    if (g->replay_reserved) return std::max(least, kWeighPieceBlocks);
+    return choose_blocks(g, runs, least, kWeighPieceBlocks, [](const LongRun& run, bool) { return run.units; });
+}
+
+// Second pass: an item for each KV head and span, through all row blocks.
+uint32_t choose_span(const psi_gqa* g, const std::vector<LongRun>& runs, bool parted) {
+    if (g->replay_reserved || parted) return kWeighSpan;
+    const uint32_t heads = g->cfg.num_kv_heads;
+    return choose_blocks(g, runs, 1, kWeighSpan, [heads](const LongRun& run, bool work) { return work ? run.units : uint64_t(heads); });
+}
+
+}  // namespace
+
 // The batch as the key-weight kernels see it (WeighRequest): short runs, their end, long runs, their end.  A batch whose
 // counts leave 32 bits is marked, and refused by psi_gqa_weigh_keys alone.
 void plan_weigh(psi_gqa* g, const uint32_t* req_slots, const uint32_t* token_indices, const uint32_t* cu_tokens, uint32_t num_reqs) {
@@ -25,41 +76,51 @@ void plan_weigh(psi_gqa* g, const uint32_t* req_slots, const uint32_t* token_ind
         w.epoch = 1;
     }
     uint64_t cu0 = 0, cu1 = 0;
+    std::vector<LongRun>& long_runs = w.long_runs;
+    long_runs.clear();
     for (int pass = 0; pass < 2; ++pass) {  // 0: short runs, 1: long ones
         cu0 = cu1 = 0;
+        const uint32_t piece_blocks = pass == 1 ? choose_piece(g, long_runs) : 0, span_blocks = pass == 1 ? choose_span(g, long_runs, w.parted) : 0;
         for (uint32_t r = 0; r < num_reqs; ++r) {
             const uint32_t q_len = cu_tokens[r + 1] - cu_tokens[r];
             if (q_len == 0) continue;
             const uint64_t rows = uint64_t(q_len) * group;
-            const bool is_short = tensor && rows <= kWeighShortRows;
-            if (is_short != (pass == 0)) continue;
-            if (w.seen[req_slots[r]] == w.epoch) w.repeated = true;
-            w.seen[req_slots[r]] = w.epoch;
             const uint32_t keys = token_indices[r] + q_len;
-            WeighRequest rq{req_slots[r], token_indices[r], q_len, cu_tokens[r], keys, uint32_t(cu0), uint32_t(cu1), uint32_t(w.long_units)};
-            w.reqs.push_back(rq);
-            w.max_keys = std::max(w.max_keys, keys);
+            const bool is_short = tensor && rows <= kWeighShortRows;
+            const uint32_t parts = is_short || g->replay_reserved
+                                       ? 1
+                                       : weigh_row_parts(static_cast<uint32_t>(std::min<uint64_t>(rows, kU32Max)), keys, heads, tensor);
+            const uint64_t units = (rows + block - 1) / block * heads;
+            if (pass == 0) {
+                if (w.seen[req_slots[r]] == w.epoch) w.repeated = true;
+                w.seen[req_slots[r]] = w.epoch;
+                w.max_keys = std::max(w.max_keys, keys);
+                if (parts > 1) w.parted = true;
+                if (!is_short && tensor) long_runs.push_back(LongRun{weigh_blocks(keys), units});
+            }
+            if (is_short != (pass == 0)) continue;
+            w.reqs.push_back(WeighRequest{req_slots[r], token_indices[r], q_len, cu_tokens[r], keys, uint32_t(cu0), uint32_t(cu1), uint32_t(w.long_units)});
             if (is_short) {
                 w.num_short += 1;
                 w.short_rows = std::max(w.short_rows, uint32_t(rows));
                 cu0 += (uint64_t(keys) + kWeighTile - 1) / kWeighTile * heads;
             } else {
                 w.num_long += 1;
-                const uint64_t units = (rows + block - 1) / block * heads;
                 w.long_units += units;
-                cu0 += units * weigh_pieces(keys, tensor);
-                const uint64_t parts = g->replay_reserved ? 1 : weigh_row_parts(static_cast<uint32_t>(std::min<uint64_t>(rows, kU32Max)), keys, heads, tensor);
-                if (parts > 1) w.parted = true;
-                cu1 += parts * weigh_spans(keys, tensor) * heads;
+                cu0 += units * (tensor ? weigh_cut(keys, piece_blocks) : weigh_any_pieces(keys));
+                cu1 += uint64_t(parts) * (tensor ? weigh_cut(keys, span_blocks) : weigh_any_spans(keys)) * heads;
             }
         }
         WeighRequest end{};
+        end.slot = piece_blocks;
+        end.first_pos = span_blocks;
         end.cu0 = uint32_t(cu0);
         end.cu1 = uint32_t(cu1);
         w.reqs.push_back(end);
         w.too_large = w.too_large || cu0 > kU32Max || cu1 > kU32Max || w.long_units > kU32Max;
         if (pass == 0) w.tiles = cu0;
     }
+    w.span_keys = tensor ? w.reqs.back().first_pos * kWeighBlock : kWeighAnyKeys;
     w.stats_items = cu0;
     w.sum_items = cu1;
     require(!w.captured || (!w.repeated && !w.too_large),
@@ -124,13 +185,14 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
             short_units = can_short ? uint64_t(g->cfg.max_tokens) * heads : 0;
             const uint64_t rows = uint64_t(g->cfg.max_tokens) * group;
             long_units = can_long ? (rows / block + (tensor ? rows / (kWeighShortRows + 1) : g->cfg.max_tokens) + 1) * heads : 0;
-            stats_items = long_units * weigh_pieces(static_cast<uint32_t>(std::min<uint64_t>(table_tokens(g), kU32Max)), tensor);
+            const uint32_t tokens = static_cast<uint32_t>(std::min<uint64_t>(table_tokens(g), kU32Max));
+            stats_items = long_units * (tensor ? std::min(weigh_cut(tokens, kWeighPieceBlocks), kWeighMaxPieces) : weigh_any_pieces(tokens));
         }
         const uint64_t short_slots = (short_ctas * 8 + short_units) * 16, long_slots = stats_items * block;
         const uint64_t partial_bytes = (short_slots + long_slots) * sizeof(float2);
         // (a span's counter stands at the place of its first item)
         const uint64_t counter_words = short_units + std::max(long_units, w.parted ? w.sum_items : 0);
-        const uint64_t sum_bytes = w.parted ? w.sum_items * weigh_span_keys(tensor) * sizeof(float) : 0;
+        const uint64_t sum_bytes = w.parted ? w.sum_items * w.span_keys * sizeof(float) : 0;
         if (ctx->capturing) {
             require(w.norms.ptr != nullptr && partial_bytes <= w.partials.bytes && counter_words * sizeof(uint32_t) <= w.counters.bytes,
                     "call psi_gqa_weigh_keys once after the replay reservation and before the capture: it allocates its scratch then");
@@ -157,7 +219,7 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
         p.counters = static_cast<uint32_t*>(w.counters.ptr);
         p.long_counters_at = short_units;
         p.sums = static_cast<float*>(w.sums.ptr);
-        p.split_rows = fixed ? 0u : 1u;
+        p.split_rows = w.parted ? 1u : 0u;
         p.group = group;
         p.short_count = fixed ? 0xFFFFFFFFu : w.num_short;
         p.short_tiles = fixed ? 0xFFFFFFFFu : static_cast<uint32_t>(w.tiles);
@@ -182,7 +244,7 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
         }
         if (ctx->capturing) w.captured = true;
         if (short_ctas > 0) run_pass(g, p, keep_scores ? WeighPass::kShortStatsScores : WeighPass::kShortStats, short_ctas);
-        const uint64_t long_wave = sms * (tensor || g->cfg.head_dim > 96 ? 2 : 4);
+        const uint64_t long_wave = tensor ? std::min<uint64_t>(weigh_wave(g->cfg.head_dim), 2 * sms) : sms * (g->cfg.head_dim > 96 ? 2 : 4);
         const uint64_t stats_ctas = fixed ? (can_long ? long_wave : 0) : std::min<uint64_t>(long_wave, w.stats_items);
         const uint64_t sum_ctas = fixed ? stats_ctas : std::min<uint64_t>(long_wave, w.sum_items);
         if (stats_ctas > 0) run_pass(g, p, WeighPass::kLongStats, stats_ctas);

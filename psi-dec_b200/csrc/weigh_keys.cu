@@ -426,10 +426,10 @@ __global__ __launch_bounds__(kAnyThreads) void weigh_stats_any_kernel(const Weig
     const uint32_t at = 2u * (threadIdx.x >> 4), column = threadIdx.x & 15u;
     for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
         const WeighRequest rq = reqs[find_request<0>(reqs, count, item)];
-        const uint32_t pieces = weigh_pieces(rq.keys, false), rows = rq.q_len * p.group, blocks = (rows + kAnyRows - 1) / kAnyRows;
+        const uint32_t pieces = weigh_any_pieces(rq.keys), rows = rq.q_len * p.group, blocks = (rows + kAnyRows - 1) / kAnyRows;
         const uint32_t local = item - rq.cu0, piece = local % pieces, unit = local / pieces;
         const uint32_t head = unit / blocks, row0 = (unit % blocks) * kAnyRows;
-        const uint32_t piece_keys = weigh_piece_keys(rq.keys, pieces);
+        const uint32_t piece_keys = weigh_any_piece_keys(rq.keys, pieces);
         const uint32_t k0 = piece * piece_keys;
         const uint32_t k1 = min(min(k0 + piece_keys, rq.keys), row_limit(p, rq, min(row0 + kAnyRows, rows) - 1));
         const uint32_t* row_ids = table_row(p.geo, rq.slot);
@@ -524,7 +524,7 @@ __global__ __launch_bounds__(kAnyThreads) void weigh_sum_any_kernel(const WeighP
     const uint32_t at = 2u * (threadIdx.x >> 4), column = threadIdx.x & 15u;
     for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
         const WeighRequest rq = reqs[find_request<1>(reqs, count, item)];
-        const uint32_t all_rows = rq.q_len * p.group, spans = weigh_spans(rq.keys, false);
+        const uint32_t all_rows = rq.q_len * p.group, spans = weigh_any_spans(rq.keys);
         const uint32_t parts = p.split_rows != 0 ? weigh_row_parts(all_rows, rq.keys, p.geo.num_kv_heads, false) : 1u;
         const uint32_t local = item - rq.cu1, part = local % parts, unit = local / parts;
         const uint32_t head = unit / spans, key0 = unit % spans * kBlock, each = weigh_part_blocks(all_rows, parts, false) * kAnyRows;

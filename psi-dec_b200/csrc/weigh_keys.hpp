@@ -10,13 +10,15 @@
 namespace psi {
 
 constexpr uint32_t kWeighBlock = 128;    // rows or keys of one block of the long-run kernels
-constexpr uint32_t kWeighSpan = 4;       // key blocks of one second-pass item of theirs
+constexpr uint32_t kWeighSpan = 4;       // key blocks of one second-pass item of theirs, where its rows are cut into parts
 constexpr uint32_t kWeighAnyRows = 32;   // rows and keys of one block of the CUDA-core kernels
 constexpr uint32_t kWeighAnyKeys = 64;
 constexpr uint32_t kWeighShortRows = 16; // query rows of a KV head up to which a run goes to the short-run kernel
 constexpr uint32_t kWeighTile = 32;      // keys of one unit of the short-run kernel's shares
-constexpr uint32_t kWeighPieceKeys = 1024, kWeighMaxPieces = 16;       // of the first pass on the tensor cores
+constexpr uint32_t kWeighPieceBlocks = 8, kWeighMaxPieces = 16;        // of the first pass on the tensor cores, replayed
 constexpr uint32_t kWeighAnyPieceKeys = 256, kWeighAnyMaxPieces = 64;  // and on the CUDA cores
+constexpr uint32_t kWeighWave = 296;     // CTAs of the long-run kernels side by side: two for each SM of a B200,
+inline uint32_t weigh_wave(uint32_t head_dim) { return head_dim <= 128 ? kWeighWave : kWeighWave / 2; }  // or one on the tensor cores
 
 // A request with tokens as the kernels see it.  Short runs first, then one entry that ends their prefix sums, then the long
 // runs and one entry that ends theirs.
@@ -29,30 +31,30 @@ struct WeighRequest {
 };
 constexpr uint64_t kWeighRequestWords = sizeof(WeighRequest) / sizeof(uint32_t);
 
-// A long run's keys are cut into a bounded number of pieces, so that the scratch does not grow with the context.
-__host__ __device__ inline uint32_t weigh_pieces(uint32_t keys, bool tensor) {
-    const uint32_t each = tensor ? kWeighPieceKeys : kWeighAnyPieceKeys, most = tensor ? kWeighMaxPieces : kWeighAnyMaxPieces;
-    const uint32_t n = keys / each + (keys % each != 0 ? 1u : 0u);
-    return n < most ? n : most;
+// The entry that ends the long runs carries, for the tensor cores, the key blocks of a first-pass piece (slot) and of a second-pass
+// span (first_pos); plan_weigh chooses them.
+__host__ __device__ inline uint32_t weigh_blocks(uint32_t keys) { return keys / kWeighBlock + (keys % kWeighBlock != 0 ? 1u : 0u); }
+__host__ __device__ inline uint32_t weigh_cut(uint32_t keys, uint32_t blocks) { return (weigh_blocks(keys) + blocks - 1) / blocks; }
+
+// CUDA cores: a long run's keys are cut into a bounded number of pieces, so that the scratch does not grow with the context.
+__host__ __device__ inline uint32_t weigh_any_pieces(uint32_t keys) {
+    const uint32_t n = keys / kWeighAnyPieceKeys + (keys % kWeighAnyPieceKeys != 0 ? 1u : 0u);
+    return n < kWeighAnyMaxPieces ? n : kWeighAnyMaxPieces;
 }
 // Keys of one piece, in whole blocks.
-__host__ __device__ inline uint32_t weigh_piece_keys(uint32_t keys, uint32_t pieces) {
+__host__ __device__ inline uint32_t weigh_any_piece_keys(uint32_t keys, uint32_t pieces) {
     const uint32_t each = keys / pieces + (keys % pieces != 0 ? 1u : 0u);
-    return (each + kWeighBlock - 1) / kWeighBlock * kWeighBlock;  // (a multiple of kWeighAnyKeys as well)
+    return (each + kWeighAnyKeys - 1) / kWeighAnyKeys * kWeighAnyKeys;
 }
+__host__ __device__ inline uint32_t weigh_any_spans(uint32_t keys) { return keys / kWeighAnyKeys + (keys % kWeighAnyKeys != 0 ? 1u : 0u); }
 
-// Second-pass spans of one KV head: blocks of keys on the tensor cores, 64 keys on the CUDA cores.
-__host__ __device__ constexpr uint32_t weigh_span_keys(bool tensor) { return tensor ? kWeighBlock * kWeighSpan : kWeighAnyKeys; }
-__host__ __device__ inline uint32_t weigh_spans(uint32_t keys, bool tensor) {
-    return keys / weigh_span_keys(tensor) + (keys % weigh_span_keys(tensor) != 0 ? 1u : 0u);
-}
 // Into how many parts a run's rows are cut in the second pass, each an item of its own whose sums the last one adds up: where the spans
-// of all KV heads are fewer than two for each SM of a B200, and a part has two row blocks left.
+// of all KV heads are fewer than two for each SM, and a part has two row blocks left.
 __host__ __device__ inline uint32_t weigh_row_parts(uint32_t rows, uint32_t keys, uint32_t heads, bool tensor) {
-    const uint64_t spans = uint64_t(weigh_spans(keys, tensor)) * heads;
-    if (spans >= 296) return 1;
+    const uint64_t spans = uint64_t(tensor ? weigh_cut(keys, kWeighSpan) : weigh_any_spans(keys)) * heads;
+    if (spans >= kWeighWave) return 1;
     const uint32_t least = tensor ? 2 * kWeighBlock : 2 * kWeighAnyRows;
-    const uint32_t wanted = uint32_t((296 + spans - 1) / spans), most = rows / least > 0 ? rows / least : 1;
+    const uint32_t wanted = uint32_t((kWeighWave + spans - 1) / spans), most = rows / least > 0 ? rows / least : 1;
     return wanted < most ? wanted : most;
 }
 // Row blocks of one part.

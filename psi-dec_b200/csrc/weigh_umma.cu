@@ -11,6 +11,8 @@
 // four prompts of 4,099 to 16,384 keys, 64 tokens of 32/8 heads x 128 each.)  Two CTAs share an SM at head_dim 128 and below, so that
 // one's loads and barriers run under the other's arithmetic.
 // Every mbarrier wait is bounded and reports PSI_ERR_TIMEOUT through the status word, and TMEM is freed on every path.
+#include <type_traits>
+
 #include "launch_util.hpp"
 #include "umma_common.cuh"
 #include "weigh_common.cuh"
@@ -61,6 +63,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks <= 2 ? 2 : 1) weigh_umma_ker
     const uint32_t count = p.scalars[kScalarWeighLong];
     const WeighRequest* reqs = p.long_reqs();
     const uint32_t total = count == 0 ? 0u : kStats ? reqs[count].cu0 : reqs[count].cu1;
+    const uint32_t cut = kStats ? reqs[count].slot : reqs[count].first_pos, cut_keys = cut * kRows;  // of an item's keys
     const uint32_t row = tid & (kRows - 1), half = tid >> 7;
     const uint32_t lane_base = ((warp & 3u) * 32u) << 16, column0 = half * (kRows / 2);
     const PageBounds bounds(p.geo);
@@ -100,31 +103,31 @@ __global__ void __launch_bounds__(kThreads, kBlocks <= 2 ? 2 : 1) weigh_umma_ker
         const uint32_t* row_ids = table_row(p.geo, rq.slot);
         uint32_t head, block_begin, block_end, k_begin, k_end, pieces = 1, unit = 0;
         if (kStats) {
-            pieces = weigh_pieces(rq.keys, true);
-            const uint32_t local = item - rq.cu0, piece = local % pieces, piece_keys = weigh_piece_keys(rq.keys, pieces);
+            pieces = weigh_cut(rq.keys, cut);
+            const uint32_t local = item - rq.cu0, piece = local % pieces;
             unit = local / pieces;
             head = unit / blocks;
             block_begin = unit % blocks;
             block_end = block_begin + 1;
-            k_begin = piece * piece_keys;
-            k_end = min(k_begin + piece_keys, rq.keys);
+            k_begin = piece * cut_keys;
+            k_end = min(k_begin + cut_keys, rq.keys);
         } else {
             pieces = p.split_rows != 0 ? weigh_row_parts(rows, rq.keys, p.geo.num_kv_heads, true) : 1u;
-            const uint32_t spans = weigh_spans(rq.keys, true), local = item - rq.cu1, part = local % pieces, each = weigh_part_blocks(rows, pieces, true);
+            const uint32_t spans = weigh_cut(rq.keys, cut), local = item - rq.cu1, part = local % pieces, each = weigh_part_blocks(rows, pieces, true);
             unit = local / pieces;
             head = unit / spans;
             block_begin = part * each;
             block_end = min(block_begin + each, blocks);
-            k_begin = unit % spans * weigh_span_keys(true);
-            k_end = min(k_begin + weigh_span_keys(true), rq.keys);
+            k_begin = unit % spans * cut_keys;
+            k_end = min(k_begin + cut_keys, rq.keys);
             // rows of tokens before the span's first key see none of it
             if (k_begin > rq.first_pos) block_begin = max(block_begin, uint32_t(uint64_t(k_begin - rq.first_pos) * p.group / kRows));
             if (pieces > 1)
-                for (uint32_t i = tid; i < weigh_span_keys(true); i += kThreads) p.sums[uint64_t(item) * weigh_span_keys(true) + i] = 0.0f;
+                for (uint32_t i = tid; i < cut_keys; i += kThreads) p.sums[uint64_t(item) * cut_keys + i] = 0.0f;
             __syncthreads();
         }
         // where a key's sum goes: its weight, or this part's share of it
-        float* const sums = kStats ? nullptr : pieces > 1 ? p.sums + uint64_t(item) * weigh_span_keys(true) - k_begin : weight_row(p, rq, head);
+        float* const sums = kStats ? nullptr : pieces > 1 ? p.sums + uint64_t(item) * cut_keys - k_begin : weight_row(p, rq, head);
         for (uint32_t block = block_begin; block < block_end; ++block) {
             const uint32_t row0 = block * kRows;
             const uint32_t seen = min(k_end, row_limit(p, rq, min(row0 + kRows, rows) - 1));  // keys that a row of the block sees end here
@@ -176,53 +179,57 @@ __global__ void __launch_bounds__(kThreads, kBlocks <= 2 ? 2 : 1) weigh_umma_ker
                         for (uint32_t c = 0; c < 64; ++c)
                             if (key + c >= my_limit) s[c] = -kInf;
                     }
-                    float top = -kInf;
+                    float tops[4] = {-kInf, -kInf, -kInf, -kInf};
 #pragma unroll
-                    for (int c = 0; c < 64; c += 2) top = max3_nan(top, s[c], s[c + 1]);  // (a NaN leaves no sum)
+                    for (int c = 0; c < 64; c += 2) tops[(c >> 1) & 3] = max3_nan(tops[(c >> 1) & 3], s[c], s[c + 1]);  // (a NaN leaves no sum)
+                    float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
                     top = max3_nan(st.m, st.m, top * p.scale_log2);
                     const float base = top == -kInf ? 0.0f : top;
                     st.l *= exp2_approx(st.m - base);
                     st.m = top;
                     const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2), base2 = pack_f32x2(-base, -base);
-                    uint64_t sum[2] = {0, 0};
+                    uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
                     for (int c = 0; c < 64; c += 2) {
                         const float2 x = unpack_f32x2(fma_f32x2(pack_f32x2(s[c], s[c + 1]), scale2, base2));
-                        sum[(c >> 1) & 1] = add_f32x2(sum[(c >> 1) & 1], pack_f32x2(exp2_approx(x.x), exp2_approx(x.y)));
+                        sum[(c >> 1) & 3] = add_f32x2(sum[(c >> 1) & 3], pack_f32x2(exp2_approx(x.x), exp2_approx(x.y)));
                     }
-                    const float2 all = unpack_f32x2(add_f32x2(sum[0], sum[1]));
+                    const float2 all = unpack_f32x2(add_f32x2(add_f32x2(sum[0], sum[1]), add_f32x2(sum[2], sum[3])));
                     st.l += all.x + all.y;
                 } else {
                     // this thread's key against 64 rows
                     const uint32_t key = key0 + row;
                     const bool masked = key0 + kRows > row_limit(p, rq, row0) || row0 + kRows > rows || sh.dead_rows != 0;
                     const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2);
-                    uint64_t sum[2] = {0, 0};
-#pragma unroll 1
-                    for (uint32_t c0 = 0; c0 < 64; c0 += 32) {
-                        float s[32];
-                        tmem_load32(at + c0, s);
+                    uint64_t sum[4] = {0, 0, 0, 0};
+                    const auto columns = [&](const auto with_mask) {
+                        float s[64];
+                        tmem_load64(at, s);
 #pragma unroll
-                        for (uint32_t c = 0; c < 32; c += 4) {
-                            const ulonglong2 base = *reinterpret_cast<const ulonglong2*>(&sh.neg_max[column0 + c0 + c]);
-                            const ulonglong2 inverse = *reinterpret_cast<const ulonglong2*>(&sh.inverse[column0 + c0 + c]);
+                        for (uint32_t c = 0; c < 64; c += 4) {
+                            const ulonglong2 base = *reinterpret_cast<const ulonglong2*>(&sh.neg_max[column0 + c]);
+                            const ulonglong2 inverse = *reinterpret_cast<const ulonglong2*>(&sh.inverse[column0 + c]);
                             float2 x = unpack_f32x2(fma_f32x2(pack_f32x2(s[c], s[c + 1]), scale2, base.x));
                             float2 y = unpack_f32x2(fma_f32x2(pack_f32x2(s[c + 2], s[c + 3]), scale2, base.y));
                             x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
                             y = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-                            if (masked) {
-                                const uint4 limit = *reinterpret_cast<const uint4*>(&sh.limit[column0 + c0 + c]);
+                            if constexpr (decltype(with_mask)::value) {
+                                const uint4 limit = *reinterpret_cast<const uint4*>(&sh.limit[column0 + c]);
                                 const float2 i0 = unpack_f32x2(inverse.x), i1 = unpack_f32x2(inverse.y);
                                 x.x = key < limit.x && i0.x > 0.0f ? x.x : 0.0f;
                                 x.y = key < limit.y && i0.y > 0.0f ? x.y : 0.0f;
                                 y.x = key < limit.z && i1.x > 0.0f ? y.x : 0.0f;
                                 y.y = key < limit.w && i1.y > 0.0f ? y.y : 0.0f;
                             }
-                            sum[0] = fma_f32x2(pack_f32x2(x.x, x.y), inverse.x, sum[0]);
-                            sum[1] = fma_f32x2(pack_f32x2(y.x, y.y), inverse.y, sum[1]);
+                            sum[c >> 2 & 1] = fma_f32x2(pack_f32x2(x.x, x.y), inverse.x, sum[c >> 2 & 1]);
+                            sum[2 + (c >> 2 & 1)] = fma_f32x2(pack_f32x2(y.x, y.y), inverse.y, sum[2 + (c >> 2 & 1)]);
                         }
-                    }
-                    const float2 all = unpack_f32x2(add_f32x2(sum[0], sum[1]));
+                    };
+                    if (masked)
+                        columns(std::true_type{});
+                    else
+                        columns(std::false_type{});
+                    const float2 all = unpack_f32x2(add_f32x2(add_f32x2(sum[0], sum[1]), add_f32x2(sum[2], sum[3])));
                     if (half == 1) sh.half[row].x = all.x + all.y;
                     asm volatile("bar.sync %0, 64;" ::"r"((warp & 3u) + 1) : "memory");  // the warps of these lanes
                     if (half == 0 && key < k_end) sums[key] += all.x + all.y + sh.half[row].x;
@@ -306,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks <= 2 ? 2 : 1) weigh_umma_ker
                     __threadfence();
                     for (uint32_t i = tid; i < k_end - k_begin; i += kThreads) {
                         float all = 0.0f;
-                        for (uint32_t o = 0; o < pieces; ++o) all += __ldcg(p.sums + uint64_t(rq.cu1 + unit * pieces + o) * weigh_span_keys(true) + i);
+                        for (uint32_t o = 0; o < pieces; ++o) all += __ldcg(p.sums + uint64_t(rq.cu1 + unit * pieces + o) * cut_keys + i);
                         weight_row(p, rq, head)[k_begin + i] += all;
                     }
                     if (tid == 0) *counter = 0;
