@@ -13,15 +13,15 @@ using LongRun = psi_weigh_plan::LongRun;
 
 // Into items of how many key blocks the long runs of a batch are cut, between `least` and kMostBlocks, on the tensor cores.  The CTAs
 // of a wave take items in turn, so that a launch takes as many rounds as items over CTAs, rounded up, of an item each; an item
-// costs kItemStart blocks beside its own (its first loads and product are exposed).  Four prompts' ends of 4,099 to 16,384 keys, 64 tokens of
-// 32/8 heads x 128: pieces of 20 blocks and spans of 9, one round each, 104 us for both passes, against 140 with 8 and 4 (2.3 rounds).
-// Batches of many runs take many rounds of whatever length: theirs is fixed.
-constexpr uint32_t kMostBlocks = 24, kItemStart = 2, kMostRuns = 64;
+// costs kItemStart blocks beside its own.  Four prompts' ends of 4,099 to 16,384 keys, 64 tokens of 32/8 heads x 128, in whole rounds:
+// 104 us for both passes, against 140 with 8 and 4 blocks an item (2.3 rounds).  Batches of many runs take many rounds of whatever
+// length: theirs is fixed.
+constexpr uint32_t kMostBlocks = 24, kItemStart = 1, kMostRuns = 64;
 
 template <typename Units>
-uint32_t choose_blocks(const psi_gqa* g, const std::vector<LongRun>& runs, uint32_t least, uint32_t otherwise, const Units& units_of) {
+uint32_t choose_blocks(const std::vector<LongRun>& runs, uint32_t least, uint32_t otherwise, const Units& units_of) {
     if (runs.size() > kMostRuns) return std::max(least, otherwise);
-    const uint32_t wave = weigh_wave(g->cfg.head_dim);
+    constexpr uint32_t wave = weigh_wave(true);
     uint32_t best = least;
     double least_cost = 1e300;
     for (uint32_t blocks = least; blocks <= std::max(least, kMostBlocks); ++blocks) {
@@ -46,14 +46,14 @@ uint32_t choose_piece(const psi_gqa* g, const std::vector<LongRun>& runs) {
     for (const LongRun& run : runs) most = std::max(most, run.key_blocks);
     const uint32_t least = (most + kWeighMaxPieces - 1) / kWeighMaxPieces;
     if (g->replay_reserved) return std::max(least, kWeighPieceBlocks);
-    return choose_blocks(g, runs, least, kWeighPieceBlocks, [](const LongRun& run, bool) { return run.units; });
+    return choose_blocks(runs, least, kWeighPieceBlocks, [](const LongRun& run, bool) { return run.units; });
 }
 
 // Second pass: an item for each KV head and span, through all row blocks.
 uint32_t choose_span(const psi_gqa* g, const std::vector<LongRun>& runs, bool parted) {
     if (g->replay_reserved || parted) return kWeighSpan;
     const uint32_t heads = g->cfg.num_kv_heads;
-    return choose_blocks(g, runs, 1, kWeighSpan, [heads](const LongRun& run, bool work) { return work ? run.units : uint64_t(heads); });
+    return choose_blocks(runs, 1, kWeighSpan, [heads](const LongRun& run, bool work) { return work ? run.units : uint64_t(heads); });
 }
 
 }  // namespace
@@ -244,7 +244,7 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
         }
         if (ctx->capturing) w.captured = true;
         if (short_ctas > 0) run_pass(g, p, keep_scores ? WeighPass::kShortStatsScores : WeighPass::kShortStats, short_ctas);
-        const uint64_t long_wave = tensor ? std::min<uint64_t>(weigh_wave(g->cfg.head_dim), 2 * sms) : sms * (g->cfg.head_dim > 96 ? 2 : 4);
+        const uint64_t long_wave = tensor ? sms : sms * (g->cfg.head_dim > 96 ? 2 : 4);
         const uint64_t stats_ctas = fixed ? (can_long ? long_wave : 0) : std::min<uint64_t>(long_wave, w.stats_items);
         const uint64_t sum_ctas = fixed ? stats_ctas : std::min<uint64_t>(long_wave, w.sum_items);
         if (stats_ctas > 0) run_pass(g, p, WeighPass::kLongStats, stats_ctas);

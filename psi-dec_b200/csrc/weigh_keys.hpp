@@ -17,8 +17,8 @@ constexpr uint32_t kWeighShortRows = 16; // query rows of a KV head up to which 
 constexpr uint32_t kWeighTile = 32;      // keys of one unit of the short-run kernel's shares
 constexpr uint32_t kWeighPieceBlocks = 8, kWeighMaxPieces = 16;        // of the first pass on the tensor cores, replayed
 constexpr uint32_t kWeighAnyPieceKeys = 256, kWeighAnyMaxPieces = 64;  // and on the CUDA cores
-constexpr uint32_t kWeighWave = 296;     // CTAs of the long-run kernels side by side: two for each SM of a B200,
-inline uint32_t weigh_wave(uint32_t head_dim) { return head_dim <= 128 ? kWeighWave : kWeighWave / 2; }  // or one on the tensor cores
+// CTAs of the long-run kernels side by side: one for each SM of a B200 on the tensor cores, two on the CUDA cores.
+__host__ __device__ constexpr uint32_t weigh_wave(bool tensor) { return tensor ? 148 : 296; }
 
 // A request with tokens as the kernels see it.  Short runs first, then one entry that ends their prefix sums, then the long
 // runs and one entry that ends theirs.
@@ -49,12 +49,12 @@ __host__ __device__ inline uint32_t weigh_any_piece_keys(uint32_t keys, uint32_t
 __host__ __device__ inline uint32_t weigh_any_spans(uint32_t keys) { return keys / kWeighAnyKeys + (keys % kWeighAnyKeys != 0 ? 1u : 0u); }
 
 // Into how many parts a run's rows are cut in the second pass, each an item of its own whose sums the last one adds up: where the spans
-// of all KV heads are fewer than two for each SM, and a part has two row blocks left.
+// of all KV heads are fewer than the CTAs of a wave, and a part has two row blocks left.
 __host__ __device__ inline uint32_t weigh_row_parts(uint32_t rows, uint32_t keys, uint32_t heads, bool tensor) {
     const uint64_t spans = uint64_t(tensor ? weigh_cut(keys, kWeighSpan) : weigh_any_spans(keys)) * heads;
-    if (spans >= kWeighWave) return 1;
+    if (spans >= weigh_wave(tensor)) return 1;
     const uint32_t least = tensor ? 2 * kWeighBlock : 2 * kWeighAnyRows;
-    const uint32_t wanted = uint32_t((kWeighWave + spans - 1) / spans), most = rows / least > 0 ? rows / least : 1;
+    const uint32_t wanted = uint32_t((weigh_wave(tensor) + spans - 1) / spans), most = rows / least > 0 ? rows / least : 1;
     return wanted < most ? wanted : most;
 }
 // Row blocks of one part.
