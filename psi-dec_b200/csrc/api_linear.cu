@@ -22,13 +22,15 @@ struct psi_linear {
 
 namespace {
 
-// Runs of more tokens take the chunked form.
-constexpr uint32_t kStepTokens = 16;
+// Runs of more tokens take the chunked form, which costs the same from 1 to 64 tokens.  16/32 heads x 128, bf16, recurrent and chunked:
+// 9 tokens 22 and 20 us, 16 tokens 28 and 19; 32 requests of 9 tokens 72 and 65 us, of 16 tokens 98 and 64.
+constexpr uint32_t kStepTokens = 8;
 
 // Into how many chunks the pieces of a batch's long runs are cut (0: nothing is cut).  The chunked form takes one CTA per run and head
 // through its chunks in turn, so that few heads leave SMs idle; pieces side by side cost a pass for the states between them.  In units
 // of a chunk's time (2.0 us at 128 x 128, the state pass's 0.5 of it): a launch takes the longest CTA's chunks, the CTAs going round
-// their items, and the scan with its two launches three.
+// their items, and the scan with its two launches three.  128 x 128, cut and whole: 32 heads, 1,024 tokens 39 and 46 us, 8,192 tokens
+// 139 and 251; 4 heads, 512 tokens 30 and 29, 1,024 tokens 31 and 45, 8,192 tokens 46 and 249.
 uint32_t piece_chunks(const std::vector<uint32_t>& run_tokens, uint32_t heads, uint32_t sms, uint32_t max_carries) {
     uint32_t longest = 0;
     const auto chunks_of = [](uint32_t tokens) { return (tokens + kLinearChunk - 1) / kLinearChunk; };

@@ -4,12 +4,14 @@
 // weight of the last kept key by a radix selection over order-preserving 32-bit keys (11, 11 and 10 bits, a histogram each, summed
 // over the cluster; it ends as soon as a digit's keys belong all or not at all), then write the kept indices in ascending order with
 // one ordered scan, which also brings the weights to their new places.  Counts are whole numbers, so ties and results do not
-// depend on the order of the atomics.  The weights are read once; the histograms and the scan bound it.
+// depend on the order of the atomics.  The weights are read once; the histograms and the scan bound it: 18 us for 64 rows of 1,024 to
+// 8,192 weights, 40 us for 16 rows of 65,001 to 131,072 on eight CTAs each.
 // evict_move_kernel / evict_move_in_place_kernel: the kept K and V rows to the front of the destination slot: bound by the
 // bytes of the rows, read and written once.  As many lanes as a row has 16-byte units take one, so that page IDs and addresses are
 // worked out once for a row.  Into another slot every row is independent.  In place a row moves to a lower or
 // equal index: a CTA takes one column slice of one head's K or V and goes through the rows in order, a batch in registers
-// between its loads and its stores, so that nothing is overwritten that a later batch reads.
+// between its loads and its stores, so that nothing is overwritten that a later batch reads.  Half of 32 caches of 1,024 to 8,192
+// keys, 2 heads x 256, bf16, into other slots: 52 us, 5.8 TB/s; a quarter of two of 65,001 to 131,072, 8 heads x 128, f32: 129 us, 6.2 TB/s.
 #include <cooperative_groups.h>
 
 #include "device_common.cuh"

