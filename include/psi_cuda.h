@@ -621,7 +621,7 @@ PSI_API int32_t psi_gqa_evict(psi_gqa* gqa, psi_pages* pages, psi_table* table, 
  * lambda = exp(log_decay),
  *   S_t = lambda S_{t-1} + k_t^T v_t,     o_t = scale q_t S_t,     S [key_dim][value_dim].
  * q and k have num_k_heads heads; value head h reads k head h / (num_v_heads / num_k_heads).  key_dim and value_dim are
- * multiples of 8 up to 256.  states: device f32 [num_req_slots][num_layers][Hv][key_dim][value_dim], the caller's,
+ * multiples of 8 up to 256, num_v_heads is 65,535 at most.  states: device f32 [num_req_slots][num_layers][Hv][key_dim][value_dim], the caller's,
  * 16-byte aligned; it needs no clearing, since a request whose token_index is 0 starts from a zero state. */
 typedef struct psi_linear_config {
     uint32_t num_k_heads;

@@ -90,6 +90,7 @@ int32_t psi_linear_create(psi_ctx* ctx, const psi_linear_config* config, psi_lin
         const psi_linear_config& c = *config;
         require(c.num_k_heads > 0 && c.num_v_heads > 0, "linear attention head counts must be positive");
         require(c.num_v_heads % c.num_k_heads == 0, "linear attention v heads must be a multiple of k heads");
+        require(c.num_v_heads <= 65535, "linear attention launches take up to 65535 v heads");
         require(c.key_dim > 0 && c.key_dim % 8 == 0 && c.key_dim <= kLinearMaxDim && c.value_dim > 0 && c.value_dim % 8 == 0 &&
                     c.value_dim <= kLinearMaxDim,
                 "linear attention key_dim and value_dim must be multiples of 8 up to 256");

@@ -16,7 +16,7 @@ using LongRun = psi_weigh_plan::LongRun;
 // costs kItemStart blocks beside its own.  Four prompts' ends of 4,099 to 16,384 keys, 64 tokens of 32/8 heads x 128, in whole rounds:
 // 104 us for both passes, against 140 with 8 and 4 blocks an item (2.3 rounds).  Batches of many runs take many rounds of whatever
 // length: theirs is fixed.
-constexpr uint32_t kMostBlocks = 24, kItemStart = 1, kMostRuns = 64;
+constexpr uint32_t kMostBlocks = 24, kItemStart = 1, kMostRuns = 16;
 
 template <typename Units>
 uint32_t choose_blocks(const std::vector<LongRun>& runs, uint32_t least, uint32_t otherwise, const Units& units_of) {

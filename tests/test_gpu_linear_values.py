@@ -127,3 +127,11 @@ def test_recurrent_and_chunked_forms_meet_at_every_length():
         s, m = by_definition(rig, 0, before, q[:n], k[:n], v[:n], [(79, 0, 4, n)])[2:]
         assert (np.abs(states[i] - s[0]) <= m[0] * 2.0 ** -24 * 300).all(), n
     rig.close()
+
+
+def test_more_heads_than_a_grid_has_rows_are_refused():
+    import torch
+    ctx = pkg.Context(0, stream=torch.cuda.current_stream().cuda_stream)
+    with pytest.raises(pkg.PsiError, match="up to 65535 v heads"):
+        pkg.LinearAttention(ctx, pkg.LinearConfig(1, 65536, 8, 8, 1.0, pkg.BF16, 1, 1, 1))
+    ctx.close()
