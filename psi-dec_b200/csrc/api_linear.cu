@@ -291,7 +291,7 @@ int32_t psi_linear_attend(psi_linear* l, uint32_t layer, float* states, const vo
         p.scale = l->cfg.scale;
         p.num_tokens = ctx->capturing ? l->cfg.max_tokens : l->num_tokens;
         p.aligned = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0 ? 1u : 0u;
-        const uint64_t wave = static_cast<uint64_t>(ctx->sm_count) * 16;
+        const uint64_t wave = static_cast<uint64_t>(ctx->sm_count) * linear_step_resident(l->cfg.key_dim);
         const uint64_t per_request = uint64_t(l->cfg.num_v_heads) * linear_step_slices(l->cfg.value_dim);
         // a captured launch has to be right for every later batch: its grid does not depend on this one
         const uint64_t items = (ctx->capturing ? uint64_t(l->cfg.max_tokens) : l->num_steps) * per_request;

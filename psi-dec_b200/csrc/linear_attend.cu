@@ -11,6 +11,7 @@
 #include "device_common.cuh"
 #include "launch_util.hpp"
 #include "linear_attend.hpp"
+#include "mma_common.cuh"
 #include "umma_common.cuh"
 
 namespace psi {
@@ -23,7 +24,9 @@ constexpr uint32_t kStepRowGroups = kStepThreads / 8;       // thread (group, fo
 constexpr uint32_t kStepTokens = 8;                         // tokens whose rows are in shared memory at once
 
 template <int kRows>  // of the state in one thread: key_dim <= 16 kRows
-__global__ __launch_bounds__(kStepThreads) void linear_step_kernel(const LinearParams p) {
+__global__ __launch_bounds__(kStepThreads, linear_step_resident(16 * kRows)) void linear_step_kernel(const LinearParams p) {
+    extern __shared__ __align__(16) unsigned char next_state[];  // of the next item; a thread reads what it copied itself
+    float4(*held)[kStepThreads] = reinterpret_cast<float4(*)[kStepThreads]>(next_state);
     __shared__ float2 rows[kStepTokens][kRows * 16];  // (k, q)
     __shared__ __align__(16) float v_cols[kStepTokens][kStepColumns];
     __shared__ __align__(16) float sums[kStepTokens][kStepThreads / 32][kStepColumns];
@@ -32,19 +35,28 @@ __global__ __launch_bounds__(kStepThreads) void linear_step_kernel(const LinearP
     const uint32_t total = p.scalars[kLinearNumSteps] * p.num_v_heads * slices;
     const uint32_t share = p.num_v_heads / p.num_k_heads;
     const uint32_t group = threadIdx.x >> 3, quad = threadIdx.x & 7u, warp = threadIdx.x >> 5;
+    const auto fetch = [&](uint32_t item) {
+        const uint32_t head = item / slices % p.num_v_heads, col = item % slices * kStepColumns + 4u * quad;
+        const LinearRequest rq = p.reqs[item / slices / p.num_v_heads];
+        const float* from = p.state_of(rq.src, head);
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) {
+            const uint32_t row = group + kStepRowGroups * j;
+            const bool there = rq.fresh == 0 && col < p.value_dim && row < p.key_dim;  // value_dim is a multiple of eight
+            cp_async_16(smem_u32(&held[j][threadIdx.x]), from + (there ? uint64_t(row) * p.value_dim + col : 0u), there ? 16u : 0u);
+        }
+        cp_async_commit();
+    };
+    if (blockIdx.x < total) fetch(blockIdx.x);
     for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
         const uint32_t slice = item % slices, head = item / slices % p.num_v_heads;
         const LinearRequest rq = p.reqs[item / slices / p.num_v_heads];
         const uint32_t col = slice * kStepColumns + 4u * quad;
-        const bool live = col < p.value_dim;  // value_dim is a multiple of eight
-        const float* from = p.state_of(rq.src, head);
+        const bool live = col < p.value_dim;
+        cp_async_wait<0>();
         ulonglong2 s[kRows];  // four columns, two in each word
 #pragma unroll
-        for (int j = 0; j < kRows; ++j) {
-            const uint32_t row = group + kStepRowGroups * j;
-            s[j] = make_ulonglong2(0, 0);
-            if (rq.fresh == 0 && live && row < p.key_dim) s[j] = *reinterpret_cast<const ulonglong2*>(from + uint64_t(row) * p.value_dim + col);
-        }
+        for (int j = 0; j < kRows; ++j) s[j] = *reinterpret_cast<const ulonglong2*>(&held[j][threadIdx.x]);
         const float hi = p.decays[head * kLinearDecays + 1], lo = p.decays[head * kLinearDecays + kLinearStepLow];
         const uint64_t hi2 = pack_f32x2(hi, hi), lo2 = pack_f32x2(lo, lo);
         for (uint32_t t0 = 0; t0 < rq.q_len; t0 += kStepTokens) {
@@ -61,6 +73,7 @@ __global__ __launch_bounds__(kStepThreads) void linear_step_kernel(const LinearP
                     c < p.value_dim ? load_as_float(p.v, (uint64_t(rq.flat_begin + t0 + t) * p.num_v_heads + head) * p.value_dim + c, p.dtype) : 0.0f;
             }
             __syncthreads();
+            if (t0 == 0 && item + gridDim.x < total) fetch(item + gridDim.x);  // (what was held has been read)
             for (uint32_t t = 0; t < tokens; ++t) {
                 const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&v_cols[t][4u * quad]);
                 uint64_t o_xy = 0, o_zw = 0;
@@ -145,10 +158,19 @@ cudaError_t launch_linear_scan(const LinearParams& p, cudaStream_t stream) {
 
 uint32_t linear_step_slices(uint32_t value_dim) { return (value_dim + kStepColumns - 1) / kStepColumns; }
 
+template <int kRows>
+static cudaError_t launch_step(const LinearParams& p, uint32_t ctas, cudaStream_t stream) {
+    constexpr int kSmem = kRows * kStepThreads * 16;
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t err = ensure_dynamic_smem(reinterpret_cast<const void*>(linear_step_kernel<kRows>), kSmem, done);
+    if (err != cudaSuccess) return err;
+    return launch_overlapped(linear_step_kernel<kRows>, dim3(ctas), dim3(kStepThreads), kSmem, stream, p);
+}
+
 cudaError_t launch_linear_step(const LinearParams& p, uint32_t ctas, cudaStream_t stream) {
-    if (p.key_dim <= 64) return launch_overlapped(linear_step_kernel<4>, dim3(ctas), dim3(kStepThreads), 0, stream, p);
-    if (p.key_dim <= 128) return launch_overlapped(linear_step_kernel<8>, dim3(ctas), dim3(kStepThreads), 0, stream, p);
-    return launch_overlapped(linear_step_kernel<16>, dim3(ctas), dim3(kStepThreads), 0, stream, p);
+    if (p.key_dim <= 64) return launch_step<4>(p, ctas, stream);
+    if (p.key_dim <= 128) return launch_step<8>(p, ctas, stream);
+    return launch_step<16>(p, ctas, stream);
 }
 
 }  // namespace psi

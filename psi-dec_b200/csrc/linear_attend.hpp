@@ -76,6 +76,8 @@ struct LinearParams {
 
 // The recurrent form, on `ctas` CTAs that take items (requests x heads x column slices) in turn; their count comes from the device.
 uint32_t linear_step_slices(uint32_t value_dim);
+// Its CTAs on an SM: what their registers leave room for.
+__host__ __device__ constexpr uint32_t linear_step_resident(uint32_t key_dim) { return key_dim <= 64 ? 9 : key_dim <= 128 ? 7 : 4; }
 cudaError_t launch_linear_step(const LinearParams& p, uint32_t ctas, cudaStream_t stream);
 // The chunked form: 16-bit types, key_dim and value_dim up to 128.
 bool linear_chunk_supported(uint32_t dtype, uint32_t key_dim, uint32_t value_dim);
