@@ -5,9 +5,12 @@
 // linear_step_kernel, the recurrent form: a CTA takes 32 columns of one head's state of one request into registers, goes through
 // the request's tokens and writes the columns back: bound by the state's bytes, read and written once for the whole run.  A
 // decay close to one that is rounded to f32 would be off by up to 2^-25 a token, and all in the same direction; it is held as two f32
-// parts instead (lambda = hi + lo to 48 bits), one more multiply-add for each element and token.  Two columns an instruction (f32x2).  One
-// token of 128 requests, 16/32 heads x 128: 100 us, 5.4 TB/s (84 % of the copy rate); four to eight tokens of 32: 45 us for 21 of
-// bytes, the arithmetic between the loads and the stores beside them.
+// parts instead (lambda = hi + lo to 48 bits), one more multiply-add for each element and token.  Two columns an instruction (f32x2).  As
+// many CTAs as are resident take items in turn, the next item's state on its way into shared memory under the one at hand, and all
+// rows of up to eight tokens are requested before the first is used.  One token of 128 requests, 16/32 heads x 128: 92 us, 5.9 TB/s (91 %
+// of the copy rate; 103 us before both); four to eight tokens of 32: 41 us for 21 of bytes, the arithmetic not quite under the transfers.
+#include <type_traits>
+
 #include "device_common.cuh"
 #include "launch_util.hpp"
 #include "linear_attend.hpp"
@@ -53,24 +56,52 @@ __global__ __launch_bounds__(kStepThreads, linear_step_resident(16 * kRows)) voi
         const LinearRequest rq = p.reqs[item / slices / p.num_v_heads];
         const uint32_t col = slice * kStepColumns + 4u * quad;
         const bool live = col < p.value_dim;
-        cp_async_wait<0>();
         ulonglong2 s[kRows];  // four columns, two in each word
-#pragma unroll
-        for (int j = 0; j < kRows; ++j) s[j] = *reinterpret_cast<const ulonglong2*>(&held[j][threadIdx.x]);
         const float hi = p.decays[head * kLinearDecays + 1], lo = p.decays[head * kLinearDecays + kLinearStepLow];
         const uint64_t hi2 = pack_f32x2(hi, hi), lo2 = pack_f32x2(lo, lo);
         for (uint32_t t0 = 0; t0 < rq.q_len; t0 += kStepTokens) {
             const uint32_t tokens = min(kStepTokens, rq.q_len - t0);
             __syncthreads();
-            for (uint32_t i = threadIdx.x; i < tokens * kRows * 16u; i += kStepThreads) {
-                const uint32_t t = i / (kRows * 16u), d = i % (kRows * 16u);
-                const uint64_t at = (uint64_t(rq.flat_begin + t0 + t) * p.num_k_heads + head / share) * p.key_dim + d;
-                rows[t][d] = d < p.key_dim ? make_float2(load_as_float(p.k, at, p.dtype), load_as_float(p.q, at, p.dtype)) : make_float2(0.0f, 0.0f);
-            }
-            for (uint32_t i = threadIdx.x; i < tokens * kStepColumns; i += kStepThreads) {
-                const uint32_t t = i / kStepColumns, c = slice * kStepColumns + i % kStepColumns;
-                v_cols[t][i % kStepColumns] =
-                    c < p.value_dim ? load_as_float(p.v, (uint64_t(rq.flat_begin + t0 + t) * p.num_v_heads + head) * p.value_dim + c, p.dtype) : 0.0f;
+            // every load of the rows is under way before the first is used
+            const auto stage = [&](const auto type, const auto most) {  // up to `most` tokens
+                constexpr uint32_t kDtype = decltype(type)::value, kMost = decltype(most)::value;
+                constexpr uint32_t kEach = (kMost * kRows * 16 + kStepThreads - 1) / kStepThreads, kEachV = (kMost * kStepColumns + kStepThreads - 1) / kStepThreads;
+                float k[kEach], q[kEach], v[kEachV];
+#pragma unroll
+                for (uint32_t n = 0; n < kEach; ++n) {
+                    const uint32_t i = threadIdx.x + n * kStepThreads, t = i / (kRows * 16u), d = i % (kRows * 16u);
+                    const bool there = t < tokens && d < p.key_dim;
+                    const uint64_t at = (uint64_t(rq.flat_begin + t0 + t) * p.num_k_heads + head / share) * p.key_dim + d;
+                    k[n] = there ? load_as_float(p.k, at, kDtype) : 0.0f;
+                    q[n] = there ? load_as_float(p.q, at, kDtype) : 0.0f;
+                }
+#pragma unroll
+                for (uint32_t n = 0; n < kEachV; ++n) {
+                    const uint32_t i = threadIdx.x + n * kStepThreads, t = i / kStepColumns, c = slice * kStepColumns + i % kStepColumns;
+                    v[n] = t < tokens && c < p.value_dim ? load_as_float(p.v, (uint64_t(rq.flat_begin + t0 + t) * p.num_v_heads + head) * p.value_dim + c, kDtype) : 0.0f;
+                }
+#pragma unroll
+                for (uint32_t n = 0; n < kEach; ++n) {
+                    const uint32_t i = threadIdx.x + n * kStepThreads;
+                    rows[i / (kRows * 16u)][i % (kRows * 16u)] = make_float2(k[n], q[n]);
+                }
+#pragma unroll
+                for (uint32_t n = 0; n < kEachV; ++n) {
+                    const uint32_t i = threadIdx.x + n * kStepThreads;
+                    v_cols[i / kStepColumns][i % kStepColumns] = v[n];
+                }
+            };
+            const auto stage_type = [&](const auto type) {
+                if (tokens == 1) stage(type, std::integral_constant<uint32_t, 1>{});
+                else stage(type, std::integral_constant<uint32_t, kStepTokens>{});
+            };
+            if (p.dtype == PSI_DTYPE_F32) stage_type(std::integral_constant<uint32_t, PSI_DTYPE_F32>{});
+            else if (p.dtype == PSI_DTYPE_BF16) stage_type(std::integral_constant<uint32_t, PSI_DTYPE_BF16>{});
+            else stage_type(std::integral_constant<uint32_t, PSI_DTYPE_F16>{});
+            if (t0 == 0) {
+                cp_async_wait<0>();
+#pragma unroll
+                for (int j = 0; j < kRows; ++j) s[j] = *reinterpret_cast<const ulonglong2*>(&held[j][threadIdx.x]);
             }
             __syncthreads();
             if (t0 == 0 && item + gridDim.x < total) fetch(item + gridDim.x);  // (what was held has been read)
@@ -86,16 +117,12 @@ __global__ __launch_bounds__(kStepThreads, linear_step_resident(16 * kRows)) voi
                     o_xy = fma_f32x2(q, s[j].x, o_xy);
                     o_zw = fma_f32x2(q, s[j].y, o_zw);
                 }
-                const float2 xy = unpack_f32x2(o_xy), zw = unpack_f32x2(o_zw);
-                float4 o = make_float4(xy.x, xy.y, zw.x, zw.y);
-#pragma unroll
-                for (int x = 8; x < 32; x <<= 1) {
-                    o.x += __shfl_xor_sync(0xFFFFFFFFu, o.x, x);
-                    o.y += __shfl_xor_sync(0xFFFFFFFFu, o.y, x);
-                    o.z += __shfl_xor_sync(0xFFFFFFFFu, o.z, x);
-                    o.w += __shfl_xor_sync(0xFFFFFFFFu, o.w, x);
-                }
-                if ((threadIdx.x & 31u) < 8u) *reinterpret_cast<float4*>(&sums[t][warp][4u * quad]) = o;
+                // over the warp's four row groups: each keeps half of what is left of the columns, and ends with one
+                const bool upper = (threadIdx.x & 16u) != 0, odd = (threadIdx.x & 8u) != 0;
+                const uint64_t theirs = __shfl_xor_sync(0xFFFFFFFFu, upper ? o_xy : o_zw, 16);
+                const float2 two = unpack_f32x2(add_f32x2(upper ? o_zw : o_xy, theirs));
+                const float one = (odd ? two.y : two.x) + __shfl_xor_sync(0xFFFFFFFFu, odd ? two.x : two.y, 8);
+                sums[t][warp][4u * quad + 2u * upper + odd] = one;
             }
             __syncthreads();
             for (uint32_t i = threadIdx.x; i < tokens * kStepColumns; i += kStepThreads) {
