@@ -23,7 +23,7 @@ struct psi_linear {
 namespace {
 
 // Runs of more tokens take the chunked form, which costs the same from 1 to 64 tokens.  16/32 heads x 128, bf16, recurrent and chunked:
-// 9 tokens 22 and 20 us, 16 tokens 28 and 19; 32 requests of 9 tokens 72 and 65 us, of 16 tokens 98 and 64.
+// 9 tokens 20 and 21 us, 16 tokens 22 and 20; 32 requests of 9 tokens 65 and 65 us, of 12 tokens 82 and 66, of 16 tokens 95 and 67.
 constexpr uint32_t kStepTokens = 8;
 
 // Into how many chunks the pieces of a batch's long runs are cut (0: nothing is cut).  The chunked form takes one CTA per run and head
