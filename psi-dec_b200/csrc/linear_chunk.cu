@@ -580,7 +580,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 mbar_arrive(bar(kBarState));
             };
             const uint32_t chunks = (run.tokens + kC - 1) / kC;
-            if constexpr (!kStateOnly) put_state(done_chunks);
             // The state after chunk `c` of the item, whose gain is complete.
             const auto advance = [&](uint32_t c) {
                 const uint32_t n = min(kC, run.tokens - c * kC);
@@ -649,6 +648,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                         }
                     }
                     fence_async_smem();
+                    __syncwarp();
+                }
+                // The state before the first chunk.  kBarState is also what the inner product waits for before it reads V: it stands
+                // behind the clearing and the removal of every chunk, the first included.
+                if constexpr (!kStateOnly) {
+                    if (c == 0) put_state(g);
                 }
                 if (c > 0) wait(kBarGain, g - 1);
                 tc_fence_after();
