@@ -9,27 +9,28 @@
 // column v of the state and of the output (accumulator lane = v), and everything that differs by v stays inside it:
 //
 //   scores   [i][j] = Q K^T                    shared memory x shared memory; lanes 64-127 are not used
-//   inner^T  [v][i] = V^T P^T                  V as it landed, P = lambda^(i-j) scores, rounded to 16 bits, in shared memory
-//   outer^T  [v][i] = S^T Q^T                  S^T rounded to 16 bits in TMEM; lambda^(i+1) is applied in f32 afterwards
-//   gain^T   [v][k] = (lambda^(n-1-j) V)^T K   the weighted V in TMEM in as many 16-bit parts as make 22 bits or more (bf16 three, f16
-//                                              two, the low one 2^11 times as large), a product each, so that the f32 state
-//                                              loses nothing to the 16-bit operands
+//   inner^T  [v][i] = V^T P^T                  V as it landed, P = lambda^(i-j) scores in shared memory, two 16-bit parts
+//   outer^T  [v][i] = S^T Q^T                  S^T in TMEM, two 16-bit parts; lambda^(i+1) is applied in f32 afterwards
+//   gain^T   [v][k] = (lambda^(n-1-j) V)^T K   the weighted V in 16-bit parts: bf16 three (24 bits, the lowest part in shared memory, the
+//                                              others in TMEM), f16 two (22 bits)
 //
-// P and S in 16 bits are two roundings of half a step of the I/O type beside the output's own: 1.4 times the error of an f32
-// product that is rounded once.  In f16 each row of P and each column of S is scaled by a power of two first, so that
-// nothing leaves f16's range.  The state itself stays in f32 registers; a chunk's gain is added to it after an
-// accumulation of its own, since the tensor cores' accumulation truncates.
+// Every part is a product of its own into the same accumulator, the lowest part first; in f16 the low part is held 2^11 times as large.
+// Two parts of P and S make 16 bits in bf16 and 22 in f16, so that an output is off by its own rounding (one part alone: 1.4 times that;
+// 8,192 tokens 142 us for 158).  In f16 each row of P and each column of S is scaled by a power of two first, so that
+// nothing leaves f16's range; the weighted V is not scaled: below 2^-14 its parts have an absolute step of 2^-35, so that
+// a state which only such values make has fewer bits than 22.  The state itself stays in f32 registers; a chunk's gain is
+// added to it after an accumulation of its own, since the tensor cores' accumulation truncates.
 //
 // Warps 0-15: four threads for each v, a quarter of the state each: weighted V (by ldmatrix, whose fragments are what tcgen05.st takes as
-// 16 x 128 bits), the state and its 16-bit copy.  Warps 16-19: outputs, in the fragments of 16 x 256 bits, which stmatrix turns into
+// 16 x 128 bits), the state and its 16-bit parts.  Warps 16-19: outputs, in the fragments of 16 x 256 bits, which stmatrix turns into
 // rows.  Warps 20 and 21: P, a row per thread.  Warp 22 issues every product but the gain, the scores a chunk ahead, so that P is made
 // under the products of the chunk before.  Warp 23 brings Q, K and V into a ring of three chunks by TMA (by plain loads where a buffer
 // is off its 16-byte boundaries; rows that the last box brings from behind a run are cleared by the state threads) and issues
 // the gains, the longest chain from chunk to chunk, which wait for the state threads alone.  The loops are kept short: unrolled, the
 // roles' code together ran out of the instruction cache and took 1.5 times as long.
-// Bound by the chain of one head's chunks, 3,500 cycles each at 128 x 128, of which the state threads work for nearly all (schedulers issue
-// in 60 % of the cycles); the products are 1,100.  One chunk of 8,192 tokens, 32 heads, f16: 140 us in pieces (42 of bytes, 10 of
-// products); three prompts of 926 to 2,185 tokens, 16/32 heads, bf16: 71 us.
+// Bound by the chain of one head's chunks, 4,000 cycles each at 128 x 128, of which the state threads work for nearly all; the
+// products are 1,500.  One prompt of 8,192 tokens, 32 heads, f16: 158 us in pieces (42 of bytes, 10 of
+// products); three prompts of 926 to 2,185 tokens, 16/32 heads, bf16: 83 us.
 // Every hand-off is an mbarrier, every wait is bounded and reports PSI_ERR_TIMEOUT through the status word, and TMEM is freed on
 // every path.
 #include <cstddef>
@@ -51,9 +52,9 @@ constexpr uint32_t kChunkThreads = (kWarpGain + 1) * 32;
 constexpr uint32_t kTileBlock = kC * 128;  // bytes of 64 rows x 64 elements
 
 // TMEM columns
-constexpr uint32_t kColScores = 0, kColInner = 64, kColOuter = 128, kColGain = 192, kColState = 320, kColParts = 384;
+constexpr uint32_t kColScores = 0, kColInner = 64, kColOuter = 128, kColGain = 192, kColState = 320, kColStateLow = 384, kColParts = 448;
 constexpr uint32_t kPartColumns = kC / 2;
-static_assert(kColParts + 3 * kPartColumns <= 512, "one TMEM allocation");
+static_assert(kColParts + 2 * kPartColumns <= 512, "one TMEM allocation");
 
 // Barriers: ring slots full and done by slot, the others one each, their phase the chunk's.  A parity wait cannot tell two
 // completions from none: a thread waits for a phase only where the next one cannot complete without it.
@@ -71,7 +72,7 @@ struct ChunkShared {
     __align__(16) float lag[4][2 * kC + 8];  // (the eight lanes of one phase of a read: distinct banks)
     // By chunk; P may be two chunks ahead of the outputs, the weighted V three.
     __align__(16) float p_scale[4][kC];       // f16: what the rows of P were divided by
-    float column_up[4][kUmmaM];               // f16: what the columns of the 16-bit state were divided by
+    float column_up[4][kUmmaM];               // f16: what the columns of the state's parts were divided by
     float column_max[2][kGroups][kUmmaM];     // f16: largest magnitude of each part of a state column
     uint32_t bad_from[4][kUmmaM];             // first token of the chunk whose V is not finite in this column (64: none)
     uint32_t any_bad;                         // the item has met such a value
@@ -115,6 +116,20 @@ __device__ __forceinline__ void split_parts(uint64_t x, uint32_t (&part)[3]) {
     }
 }
 
+// The same in two parts: bf16 the first towards zero, f16 the second 2^11 times as large.
+template <typename T>
+__device__ __forceinline__ void split_two(uint64_t x, uint32_t& high, uint32_t& low) {
+    float2 v = unpack_f32x2(x);
+    if constexpr (kIsHalf<T>) {
+        high = Mma<T>::pack(v.x, v.y);
+        v = unpack_f32x2(mul_f32x2(rest_of(x, Mma<T>::unpack(high)), pack_f32x2(2048.0f, 2048.0f)));
+    } else {
+        high = Mma<T>::pack_down(v.x, v.y);
+        v = unpack_f32x2(rest_of(x, Mma<T>::unpack(high)));
+    }
+    low = Mma<T>::pack(v.x, v.y);
+}
+
 // Byte offset of the 16-byte chunk `chunk` of row `row` in a tile of 64 rows: 64-element blocks one after another, each in the
 // 128-byte swizzle.
 __device__ __forceinline__ uint32_t tile_offset(uint32_t row, uint32_t chunk) {
@@ -130,16 +145,10 @@ __device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* m
         : "memory");
 }
 
-template <int N>
-__device__ __forceinline__ void tmem_store_bits(uint32_t taddr, const uint32_t (&v)[N]) {
-    if constexpr (N == 16) {
-        tmem_store16_bits(taddr, v);
-    } else {
-        static_assert(N == 8, "eight or sixteen columns");
-        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-                     "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                     : "memory");
-    }
+__device__ __forceinline__ void tmem_store8_bits(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 
 // 16 lanes x 8 columns as fragments: register 2 b + h of lane t is row t / 4 + 8 h, column 4 b + t % 4.
@@ -171,6 +180,14 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uin
     asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+__device__ __forceinline__ void stmatrix_x4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+__device__ __forceinline__ void st_shared16(uint32_t addr, const uint32_t (&v)[4]) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+
 __device__ __forceinline__ void st_shared_zero16(uint32_t addr) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(addr), "r"(0u) : "memory");
 }
@@ -194,7 +211,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t smem_p = smem_base + kStages * kStageBytes, smem_out = smem_p + 2 * kTileBlock;
+    const uint32_t smem_p = smem_base + kStages * kStageBytes, smem_out = smem_p + 4 * kTileBlock, smem_low = smem_out + 2 * kTileBlock;
     const uint32_t bar0 = smem_u32(shared.bars);
     const auto bar = [&](uint32_t which) { return bar0 + which * 8u; };
     if (warp == 0) {
@@ -254,13 +271,22 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                         wait(kBarState, h);
                         if (h > 0) wait(kBarOut, h - 1);
                         tc_fence_after();
-                        const uint64_t q_rows = umma_desc(stage_of(h), 16, 1024), p_rows = umma_desc(smem_p + (h & 1u) * kTileBlock, 16, 1024),
+                        const uint64_t q_rows = umma_desc(stage_of(h), 16, 1024), p_rows = umma_desc(smem_p + (h & 1u) * (2 * kTileBlock), 16, 1024),
                                        v_cols = umma_desc(stage_of(h) + 2 * kQBytes, kTileBlock, 1024);
                         if (elect_one()) {
 #pragma unroll
-                            for (uint32_t ks = 0; ks < DK / 16; ++ks) umma_ts(tmem + kColOuter, tmem + kColState + ks * 8, q_rows + row_step(ks), id_rows, ks);
+                            for (uint32_t ks = 0; ks < DK / 16; ++ks) umma_ts(tmem + kColOuter, tmem + kColStateLow + ks * 8, q_rows + row_step(ks), id_rows, ks);
+                            if (kIsHalf<T>) umma_ts_down11(tmem + kColOuter, tmem + kColState, q_rows, id_rows);
+                            else umma_ts(tmem + kColOuter, tmem + kColState, q_rows, id_rows, 1u);
 #pragma unroll
-                            for (uint32_t ks = 0; ks < kC / 16; ++ks) umma_ss(tmem + kColInner, v_cols + ks * 2048 / 16, p_rows + ks * 2, id_inner, ks);
+                            for (uint32_t ks = 1; ks < DK / 16; ++ks) umma_ts(tmem + kColOuter, tmem + kColState + ks * 8, q_rows + row_step(ks), id_rows, 1u);
+#pragma unroll
+                            for (uint32_t ks = 0; ks < kC / 16; ++ks)
+                                umma_ss(tmem + kColInner, v_cols + ks * 2048 / 16, p_rows + kTileBlock / 16 + ks * 2, id_inner, ks);
+                            if (kIsHalf<T>) umma_ss_down11(tmem + kColInner, v_cols, p_rows, id_inner);
+                            else umma_ss(tmem + kColInner, v_cols, p_rows, id_inner, 1u);
+#pragma unroll
+                            for (uint32_t ks = 1; ks < kC / 16; ++ks) umma_ss(tmem + kColInner, v_cols + ks * 2048 / 16, p_rows + ks * 2, id_inner, 1u);
                             umma_commit_one(bar(kBarDone + h % kStages));
                         }
                         __syncwarp();
@@ -333,11 +359,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 if (g > 0) wait(kBarGainRead, g - 1);
                 tc_fence_after();
                 if (elect_one()) {
+                    // the lowest part first
+                    if constexpr (!kIsHalf<T>) {
+                        const uint64_t low = umma_desc(smem_low, 16, 1024);
 #pragma unroll
-                    for (int part = int(kParts) - 1; part >= 0; --part) {  // the lowest part first
+                        for (uint32_t ks = 0; ks < kC / 16; ++ks) umma_ss(tmem + kColGain, low + ks * 2, k_cols + ks * 2048 / 16, id_gain, ks);
+                    }
+#pragma unroll
+                    for (int part = 1; part >= 0; --part) {
                         const uint32_t first = tmem + kColParts + part * kPartColumns;
                         if (kIsHalf<T> && part == 0) umma_ts_down11(tmem + kColGain, first, k_cols, id_gain);
-                        else umma_ts(tmem + kColGain, first, k_cols, id_gain, part < int(kParts) - 1 ? 1u : 0u);
+                        else umma_ts(tmem + kColGain, first, k_cols, id_gain, part == 0 || !kIsHalf<T> ? 1u : 0u);
 #pragma unroll
                         for (uint32_t ks = 1; ks < kC / 16; ++ks) umma_ts(tmem + kColGain, first + ks * 8, k_cols + ks * 2048 / 16, id_gain, 1u);
                     }
@@ -394,24 +426,30 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                         shared.p_scale[g & 3u][row] = up;
                     }
                     if (g >= 2) wait(kBarDone + (g - 2) % kStages, (g - 2) / kStages);  // the product that read this half of the buffer
-                    const uint32_t tile = smem_p + (g & 1u) * kTileBlock;
+                    const uint32_t tile = smem_p + (g & 1u) * (2 * kTileBlock);
 #pragma unroll 1
                     for (uint32_t j0 = 0; j0 < end; j0 += 16) {
                         float x[16];
                         take(j0, x);
 #pragma unroll
                         for (uint32_t y = 0; y < 16; y += 8) {
-                            if constexpr (kIsHalf<T>) {
+                            uint32_t high[4], low[4];
 #pragma unroll
-                                for (uint32_t j = y; j < y + 8; ++j) x[j] *= down;
+                            for (uint32_t j = 0; j < 4; ++j) {
+                                uint64_t two = pack_f32x2(x[y + 2 * j], x[y + 2 * j + 1]);
+                                if constexpr (kIsHalf<T>) two = mul_f32x2(two, pack_f32x2(down, down));
+                                split_two<T>(two, high[j], low[j]);
                             }
-                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(tile + tile_offset(row, (j0 + y) / 8)), "r"(Mma<T>::pack(x[y], x[y + 1])),
-                                         "r"(Mma<T>::pack(x[y + 2], x[y + 3])), "r"(Mma<T>::pack(x[y + 4], x[y + 5])), "r"(Mma<T>::pack(x[y + 6], x[y + 7]))
-                                         : "memory");
+                            const uint32_t to = tile + tile_offset(row, (j0 + y) / 8);
+                            st_shared16(to, high);
+                            st_shared16(to + kTileBlock, low);
                         }
                     }
 #pragma unroll 1
-                    for (uint32_t x = end / 8; x < 8; ++x) st_shared_zero16(tile + tile_offset(row, x));
+                    for (uint32_t x = end / 8; x < 8; ++x) {
+                        st_shared_zero16(tile + tile_offset(row, x));
+                        st_shared_zero16(tile + kTileBlock + tile_offset(row, x));
+                    }
                     fence_async_smem();
                     tc_fence_before();
                     mbar_arrive(bar(kBarP));
@@ -436,9 +474,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     const uint32_t g = done_chunks + c, n = min(kC, run.tokens - c * kC);
                     wait(kBarDone + g % kStages, g / kStages);
                     tc_fence_after();
+                    asm volatile("bar.sync 7, %0;" ::"n"(kOutThreads) : "memory");  // the rows of the chunk before have been read
                     // [token][v] in shared memory, 16 columns v and 32 tokens at a time: lane t gives the address of row t % 8 (a token)
                     // of matrix t / 8 (8 tokens x 8 columns: two of columns, then of tokens)
-                    const uint32_t tile = smem_out + (g & 1u) * (2 * kTileBlock);
+                    const uint32_t tile = smem_out;
                     const bool any_bad = *reinterpret_cast<volatile uint32_t*>(&shared.any_bad) != 0;
 #pragma unroll 1
                     for (uint32_t half = 0; half < 2; ++half) {
@@ -488,7 +527,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     }
                     tc_fence_before();
                     mbar_arrive(bar(kBarOut));
-                    // (whoever writes to this buffer again has met the readers at the next chunk's barrier)
                     asm volatile("bar.sync 7, %0;" ::"n"(kOutThreads) : "memory");
                     const uint32_t column = thread & 15u;
                     if (column * 8 < p.value_dim) {
@@ -568,13 +606,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     range_scale(largest, down, up);
                     if (group == 0) shared.column_up[g & 3u][v] = up;
                 }
-                uint32_t packed[kRows / 2];
 #pragma unroll
-                for (uint32_t k = 0; k < kRows / 2; ++k) {
-                    const float2 two = unpack_f32x2(kIsHalf<T> ? mul_f32x2(s[k], pack_f32x2(down, down)) : s[k]);
-                    packed[k] = Mma<T>::pack(two.x, two.y);
+                for (uint32_t k = 0; k < kRows / 2; k += 8) {
+                    uint32_t high[8], low[8];
+#pragma unroll
+                    for (uint32_t x = 0; x < 8; ++x) split_two<T>(kIsHalf<T> ? mul_f32x2(s[k + x], pack_f32x2(down, down)) : s[k + x], high[x], low[x]);
+                    tmem_store8_bits(tmem + kColState + lane_base + k0 / 2 + k, high);
+                    tmem_store8_bits(tmem + kColStateLow + lane_base + k0 / 2 + k, low);
                 }
-                tmem_store_bits(tmem + kColState + lane_base + k0 / 2, packed);
                 tmem_store_wait();
                 tc_fence_before();
                 mbar_arrive(bar(kBarState));
@@ -659,9 +698,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 tc_fence_after();
                 const uint32_t parts_at = tmem + kColParts + lane_base + token0 / 2;
 #pragma unroll
-                for (uint32_t x = 0; x < kParts; ++x) {
+                for (uint32_t x = 0; x < 2; ++x) {
                     tmem_store_16x128_x2(parts_at + x * kPartColumns, parts[x][0]);
                     tmem_store_16x128_x2(parts_at + x * kPartColumns + (16u << 16), parts[x][1]);
+                }
+                if constexpr (kParts == 3) {  // [v][token] in shared memory: lane t gives the address of its column v's row
+#pragma unroll
+                    for (uint32_t b = 0; b < kGroupTokens / 8; ++b)
+                        stmatrix_x4(smem_low + tile_offset(v, token0 / 8 + b), parts[2][0][2 * b], parts[2][0][2 * b + 1], parts[2][1][2 * b], parts[2][1][2 * b + 1]);
+                    fence_async_smem();
                 }
                 tmem_store_wait();
                 tc_fence_before();
@@ -703,7 +748,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 
 template <typename T, uint32_t DK, bool kStateOnly>
 cudaError_t launch_one(const LinearParams& params, uint32_t ctas, cudaStream_t stream) {
-    constexpr int kSmem = int(kStages * (2 * (DK / 64) + 2) * kTileBlock + 2 * kTileBlock + 4 * kTileBlock + 1024);
+    // the ring, P in two parts twice, the outputs, V's lowest part (bf16)
+    constexpr int kSmem = int((kStages * (2 * (DK / 64) + 2) + 4 + 2 + (kIsHalf<T> ? 0 : 2)) * kTileBlock + 1024);
+    static_assert(kSmem + sizeof(ChunkShared) <= 227 * 1024);
     LinearParams p = params;
     CUtensorMap q_map{}, k_map{}, v_map{};
     p.aligned = p.aligned != 0 && make_rows_map(p.q, p.dtype, p.key_dim, p.num_k_heads, p.num_tokens, kC, &q_map) &&

@@ -195,9 +195,14 @@ __device__ __forceinline__ void umma_ss(uint32_t tmem_d, uint64_t a, uint64_t b,
                  "r"(idesc), "r"(accumulate)
                  : "memory");
 }
-// umma_ts that adds to 2^-11 times what the accumulator holds.
+// The two that add to 2^-11 times what the accumulator holds.
 __device__ __forceinline__ void umma_ts_down11(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 1, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p, 11;\n\t}\n" ::"r"(tmem_d), "r"(tmem_a),
+                 "l"(b), "r"(idesc)
+                 : "memory");
+}
+__device__ __forceinline__ void umma_ss_down11(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 1, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p, 11;\n\t}\n" ::"r"(tmem_d), "l"(a),
                  "l"(b), "r"(idesc)
                  : "memory");
 }
