@@ -422,9 +422,15 @@ PSI_API int32_t psi_gqa_set_norm_rope(psi_gqa* gqa, const psi_norm_rope_config* 
 /* The three stages GQA::record puts before the attention (backend.rs:465-513: q norm/rope, k norm/rope,
  * kv_page_write; shaders metal/rms_norm_rope.metal, metal/gqa_kv_page_write.metal) as ONE launch: q_out receives the
  * normalised, rotated queries, the normalised, rotated keys go straight into their pages (no k scratch), the values
- * are copied into theirs.  q_in/q_out [T][Hq][D], k_in/v_in [T][Hkv][D], device, positions = the prepared batch. */
+ * are copied into theirs.  q_in/q_out [T][Hq][D], k_in/v_in [T][Hkv][D], device, positions = the prepared batch: a token goes to its
+ * token index and is rotated by it, or by the position that psi_gqa_set_positions gave. */
 PSI_API int32_t psi_gqa_norm_rope_append(psi_gqa* gqa, psi_pages* pages, psi_table* table, uint32_t layer,
                                          const void* q_in, const void* k_in, const void* v_in, void* q_out);
+/* Rotary positions of the prepared batch, where they are not its token indices (a cache that psi_gqa_evict cut): token i of request
+ * r is rotated by positions[r] + i, below 2^24, in psi_gqa_norm_rope_append and psi_gqa_projection_norm_rope_append.  Host array
+ * with an entry for each request that was prepared; holds until the next psi_gqa_prepare, after which positions are the token
+ * indices again.  Needs psi_gqa_set_norm_rope; stays outside stream captures, whose launches follow it from step to step. */
+PSI_API int32_t psi_gqa_set_positions(psi_gqa* gqa, const uint32_t* positions, uint32_t num_reqs);
 /* psi_gqa_norm_rope_append reading q, k and v (and the gates) where the fused projection left them, which also
  * removes the de-interleave stage GQA::record puts in front of them (backend.rs:449-464; GQAQGKVSplitKernel,
  * crates/inference-backend-metal/src/components/gqa_qgkv_split.rs:152-200 with metal/gqa_qgkv_split.metal:14-42, and
@@ -608,7 +614,8 @@ PSI_API int32_t psi_gqa_weigh_keys(psi_gqa* gqa, psi_pages* pages, psi_table* ta
  * one position: kept, device u32 [num_reqs][Hkv][kept_stride], receives the old indices in ascending order; entries beyond
  * keeps[r] are left.  weights_out (same shape as weights, may be the same buffer) receives at [dst slot][head] the kept
  * keys' weights and zeros for [keeps[r], lengths[r]).  Keys are cached after their rotation, so kept rows stay valid; the
- * request's next token has token index keeps[r] in psi_gqa_prepare (and its true position wherever it is rotated).  Pages behind the last kept
+ * request's next token has token index keeps[r] in psi_gqa_prepare, and is rotated by its true position: every later step of a
+ * request that was cut gives it to psi_gqa_set_positions where the library rotates.  Pages behind the last kept
  * token are the caller's to free.  src_slots, dst_slots, lengths, keeps: host arrays, read before the call returns.  A slot
  * may be a source once and a destination once, and a destination is no other request's source.  Works without a prepared
  * batch; not inside a stream capture. */

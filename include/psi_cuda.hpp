@@ -374,6 +374,10 @@ public:
                                         cu_tokens.data(), static_cast<uint32_t>(req_slots.size()), k_host, v_host, q_host,
                                         out_host), ctx_);
     }
+    // Rotary positions of the prepared batch's requests, where they are not its token indices; until the next prepare.
+    void set_positions(const std::vector<uint32_t>& positions) {
+        detail::check(psi_gqa_set_positions(handle(), positions.data(), static_cast<uint32_t>(positions.size())), ctx_);
+    }
     // Adds the attention weight that the prepared batch's queries give each cached key to weights, device f32
     // [num_req_slots][Hkv][weights_stride].
     void weigh_keys(PageArena& pages, GQARequestPageTable& table, uint32_t layer, const void* q, float* weights,

@@ -698,6 +698,12 @@ class GQA:
         _check(library().psi_gqa_decode_step_host(self._h, pages._h, table._h, C.c_uint32(layer), _ptr(k_host),
                                                   _ptr(v_host), _ptr(q_host), _ptr(out_host)), self.ctx._h)
 
+    def set_positions(self, positions):
+        """Rotary positions of the prepared batch's requests (each one's first token), where they are not its token indices: after
+        an eviction.  They hold until the next prepare."""
+        values, n = _u32_array(positions)
+        _check(library().psi_gqa_set_positions(self._h, values, C.c_uint32(n)), self.ctx._h)
+
     def weigh_keys(self, pages: PageArena, table: GQARequestPageTable, layer: int, q, weights, weights_stride: int):
         """Add the attention weight that each cached key gathers from the prepared batch's queries to ``weights``
         (f32 ``[num_req_slots][Hkv][weights_stride]``)."""

@@ -445,6 +445,7 @@ void prepare_impl(psi_gqa* g, const uint32_t* req_slots, const uint32_t* token_i
             cuda_check(cudaEventRecord(g->upload_done, ctx->stream), "cudaEventRecord");
         }
 
+        g->batch_cu.assign(cu_tokens, cu_tokens + num_reqs + 1);
         g->shape = shape;
         g->variant = variant;
         g->prepared = true;

@@ -3,6 +3,10 @@
 
 using namespace psi;
 
+namespace {
+constexpr uint64_t kMostPositions = 1ull << 24;
+}
+
 extern "C" {
 
 int32_t psi_gqa_create(psi_ctx* ctx, const psi_gqa_config* config, psi_gqa** out) {
@@ -71,6 +75,9 @@ int32_t psi_gqa_destroy(psi_gqa* g) {
         g->sync_words.release();
         g->xchg_local.release();
         g->norm_rope.release();
+        g->positions.release();
+        if (g->positions_staging != nullptr) (void)cudaFreeHost(g->positions_staging);
+        if (g->positions_done != nullptr) (void)cudaEventDestroy(g->positions_done);
         g->weigh.norms.release();
         g->weigh.partials.release();
         g->weigh.counters.release();
@@ -301,11 +308,43 @@ int32_t psi_gqa_set_norm_rope(psi_gqa* g, const psi_norm_rope_config* config, co
         std::memcpy(host.data() + 2 * weight_bytes, params.inverse_frequencies.data(),
                     params.inverse_frequencies.size() * sizeof(float));
         g->norm_rope.ensure(ctx, host.size(), false);
+        const uint64_t tokens = g->cfg.max_tokens;
+        g->positions.ensure(ctx, tokens * sizeof(uint32_t), false);
+        if (g->positions_staging == nullptr)
+            cuda_check(cudaMallocHost(reinterpret_cast<void**>(&g->positions_staging), (tokens + 1) * sizeof(uint32_t)), "cudaMallocHost");
+        if (g->positions_done == nullptr)
+            cuda_check(cudaEventCreateWithFlags(&g->positions_done, cudaEventDisableTiming), "cudaEventCreateWithFlags");
         cuda_check(cudaMemcpyAsync(g->norm_rope.ptr, host.data(), host.size(), cudaMemcpyHostToDevice, ctx->stream),
                    "cudaMemcpyAsync");  // pageable source: staged before the call returns
         g->norm_rope_cfg = *config;
         g->norm_rope_attention_factor = params.attention_factor;
         g->has_norm_rope = true;
+    });
+}
+
+int32_t psi_gqa_set_positions(psi_gqa* g, const uint32_t* positions, uint32_t num_reqs) {
+    if (g == nullptr) return PSI_ERR_INVALID_ARGUMENT;
+    return guarded(g->ctx, [&] {
+        psi_ctx* ctx = g->ctx;
+        require(g->prepared, "GQA batch metadata must be updated before its positions");
+        require(g->has_norm_rope, "psi_gqa_set_norm_rope must be called before psi_gqa_set_positions");
+        require(!ctx->capturing, "psi_gqa_set_positions uploads the step's positions and stays outside captured graphs");
+        require(positions != nullptr, "positions must not be null");
+        const std::vector<uint32_t>& cu = g->batch_cu;
+        require(num_reqs + 1ull == cu.size(), "positions must name every request of the prepared batch");
+        for (uint32_t r = 0; r < num_reqs; ++r)
+            require(uint64_t(positions[r]) + (cu[r + 1] - cu[r]) <= kMostPositions, "rotary positions must stay below 2^24, where f32 holds them");
+        ctx->bind();
+        cuda_check(cudaEventSynchronize(g->positions_done), "cudaEventSynchronize");  // previous upload left staging
+        uint32_t* s = g->positions_staging;
+        for (uint32_t r = 0; r < num_reqs; ++r)
+            for (uint32_t t = cu[r]; t < cu[r + 1]; ++t) s[t] = positions[r] + (t - cu[r]);
+        uint32_t* flag = s + g->cfg.max_tokens;
+        *flag = 1;
+        cuda_check(cudaMemcpyAsync(g->positions.ptr, s, cu.back() * sizeof(uint32_t), cudaMemcpyHostToDevice, ctx->stream), "cudaMemcpyAsync");
+        cuda_check(cudaMemcpyAsync(static_cast<uint32_t*>(g->block.ptr) + kScalarPositions, flag, sizeof(uint32_t), cudaMemcpyHostToDevice, ctx->stream),
+                   "cudaMemcpyAsync");
+        cuda_check(cudaEventRecord(g->positions_done, ctx->stream), "cudaEventRecord");
     });
 }
 
@@ -327,6 +366,7 @@ PrepParams norm_rope_params(psi_gqa* g, psi_pages* pages, psi_table* table, uint
     p.dtype = g->cfg.dtype;
     p.req_slots = block_words(g, g->off_req_slots);
     p.flat_token_indices = block_words(g, g->off_token_indices);
+    p.positions = static_cast<const uint32_t*>(g->positions.ptr);
     p.scalars = block_words(g, 0);
     p.num_total_tokens = g->shape.num_total_tokens;
     return p;

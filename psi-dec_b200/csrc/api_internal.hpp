@@ -266,6 +266,10 @@ struct psi_gqa {
     psi_norm_rope_config norm_rope_cfg{};
     float norm_rope_attention_factor = 1.0f;
     bool has_norm_rope = false;
+    psi::DeviceBuffer positions;          // [max_tokens]: rotary positions of the prepared batch's tokens, where they were given
+    uint32_t* positions_staging = nullptr;  // the same and the word that says so
+    cudaEvent_t positions_done = nullptr;
+    std::vector<uint32_t> batch_cu;       // cu_tokens of the prepared batch
     psi_weigh_plan weigh;
 };
 

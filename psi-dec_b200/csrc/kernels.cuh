@@ -18,6 +18,7 @@ enum ScalarSlot : uint32_t {
     kScalarFineChunks = 4,        // the chunk plan's items want their weights in two parts (tcgen05 kernel)
     kScalarWeighShort = 5,        // key weights: requests on the short-run kernel, and on the long-run kernels
     kScalarWeighLong = 6,
+    kScalarPositions = 7,         // the front stage rotates by positions of their own instead of the token indices
     kScalarCount = 8
 };
 
@@ -63,6 +64,7 @@ struct PrepParams {
     uint32_t dtype;
     const uint32_t* req_slots;
     const uint32_t* flat_token_indices;
+    const uint32_t* positions;    // of each token, where kScalarPositions says so
     const uint32_t* scalars;
     uint32_t num_total_tokens;
     // Source strides in elements: row (token, head) of q starts at token * q_token_stride + head * q_head_stride, of

@@ -36,6 +36,11 @@ __device__ __forceinline__ void copy_element(void* dst, uint64_t dst_index, cons
     }
 }
 
+// What a token is rotated by.
+__device__ __forceinline__ float rotary_position(const PrepParams& p, uint32_t token, uint32_t index) {
+    return static_cast<float>(p.scalars[kScalarPositions] != 0 ? p.positions[token] : index);
+}
+
 template <uint32_t DTYPE>
 __global__ void __launch_bounds__(kPrepWarps * 32) norm_rope_append_kernel(PrepParams p) {
     await_previous_kernel();
@@ -88,7 +93,7 @@ __global__ void __launch_bounds__(kPrepWarps * 32) norm_rope_append_kernel(PrepP
     acc = warp_sum(acc);
     const float inv_rms = 1.0f / sqrtf(acc / static_cast<float>(D) + p.eps);
     const __nv_bfloat16* weight = reinterpret_cast<const __nv_bfloat16*>(is_q ? p.q_weight : p.k_weight);
-    const float position = static_cast<float>(p.flat_token_indices[token]);
+    const float position = rotary_position(p, token, p.flat_token_indices[token]);
     const uint32_t rope_half = p.rope_dim / 2;
     auto normed = [&](uint32_t d) {
         const float w = round_to<DTYPE>(__bfloat162float(weight[d]));
@@ -239,9 +244,10 @@ __global__ void __launch_bounds__(kPrepWarps * 32, DTYPE == PSI_DTYPE_F32 ? 3 : 
     auto find_page = [&] { page_ok = checked_page_id(p.geo, table_row(p.geo, slot), pos / p.geo.tokens_per_page, page_id); };
     if (p.geo.table_settled != 0) find_page();
     const uint32_t rope_half = p.rope_dim / 2, half_lanes = rope_half / 8;
+    const float position = rotary_position(p, token, pos);
     for (uint32_t i = tid; i < rope_half; i += kPrepWarps * 32) {
         float s, c;
-        sincosf(static_cast<float>(pos) * p.inverse_frequencies[i], &s, &c);
+        sincosf(position * p.inverse_frequencies[i], &s, &c);
         turn_s[i] = make_float2(c, s);
     }
     await_previous_kernel();
