@@ -342,7 +342,10 @@ void prepare_impl(psi_gqa* g, const uint32_t* req_slots, const uint32_t* token_i
                     "GQA request context does not fit the request page table");
         }
 
-        plan_weigh(g, req_slots, token_indices, cu_tokens, num_reqs);
+        psi_weigh_plan& weigh = g->weigh;
+        weigh.planned = false;
+        if (weigh.wanted) plan_weigh(g, req_slots, token_indices, cu_tokens, num_reqs);
+        const uint64_t weigh_words = (weigh.wanted ? weigh.reqs.size() : num_reqs + 2ull) * kWeighRequestWords;
         if (g->cfg.plan_mode == PSI_PLAN_REFERENCE) {
             g->plan = build_reference_plan(g->geo, *g->md, shape, variant.tiled_q != 0, token_indices, cu_tokens,
                                            num_reqs);
@@ -383,23 +386,23 @@ void prepare_impl(psi_gqa* g, const uint32_t* req_slots, const uint32_t* token_i
             cursor += pad_words(num_tokens);
             g->off_token_indices = cursor;
             cursor += pad_words(num_tokens);
-            g->off_weigh = cursor;
-            cursor += g->weigh.reqs.size() * kWeighRequestWords;
             place_plan(g->off, cursor, plan, chunk, device_items.size());
             if (g->has_merged) {
                 g->merged_off.scalars = cursor;
                 cursor += pad_words(kScalarCount);
                 place_plan(g->merged_off, cursor, g->merged_plan, g->merged_chunk, merged_items.size());
             }
-            words = cursor;
+            g->off_weigh = cursor;  // last: there is room for it where nothing is uploaded yet
+            const uint64_t whole = cursor + weigh_words;
+            words = weigh.wanted ? whole : cursor;
 
-            if (g->staging_words < words) {
+            if (g->staging_words < whole) {
                 if (g->staging != nullptr) {
                     cuda_check(cudaEventSynchronize(g->upload_done), "cudaEventSynchronize");
                     cuda_check(cudaFreeHost(g->staging), "cudaFreeHost");
                     g->staging = nullptr;
                 }
-                const uint64_t grown = std::max<uint64_t>(words * 2, 4096);
+                const uint64_t grown = std::max<uint64_t>(whole * 2, 4096);
                 cuda_check(cudaMallocHost(reinterpret_cast<void**>(&g->staging), grown * sizeof(uint32_t)), "cudaMallocHost");
                 g->staging_words = grown;
             } else {
@@ -422,9 +425,15 @@ void prepare_impl(psi_gqa* g, const uint32_t* req_slots, const uint32_t* token_i
         std::copy(g->md->req_slots.begin(), g->md->req_slots.begin() + num_tokens, s + g->off_req_slots);
         std::copy(g->md->flat_token_indices.begin(), g->md->flat_token_indices.begin() + num_tokens,
                   s + g->off_token_indices);
-        s[kScalarWeighShort] = g->weigh.num_short;
-        s[kScalarWeighLong] = g->weigh.num_long;
-        std::memcpy(s + g->off_weigh, g->weigh.reqs.data(), g->weigh.reqs.size() * sizeof(WeighRequest));
+        if (weigh.wanted) {
+            s[kScalarWeighShort] = weigh.num_short;
+            s[kScalarWeighLong] = weigh.num_long;
+            std::memcpy(s + g->off_weigh, weigh.reqs.data(), weigh_words * sizeof(uint32_t));
+            if (g->replay_reserved)  // behind the prefix that is uploaded below
+                cuda_check(cudaMemcpyAsync(static_cast<uint32_t*>(g->block.ptr) + g->off_weigh, s + g->off_weigh, weigh_words * sizeof(uint32_t), cudaMemcpyHostToDevice,
+                                           ctx->stream),
+                           "cudaMemcpyAsync");
+        }
         if (g->replay_reserved) {
             // launches run at the capacity grid: CTAs beyond the plan's find an empty range and a zero first item
             constexpr uint64_t kItemWords = sizeof(DeviceItem) / sizeof(uint32_t);
@@ -446,6 +455,9 @@ void prepare_impl(psi_gqa* g, const uint32_t* req_slots, const uint32_t* token_i
         }
 
         g->batch_cu.assign(cu_tokens, cu_tokens + num_reqs + 1);
+        weigh.batch_slots.assign(req_slots, req_slots + num_reqs);
+        weigh.batch_tokens.assign(token_indices, token_indices + num_reqs);
+        weigh.planned = weigh.wanted;
         g->shape = shape;
         g->variant = variant;
         g->prepared = true;

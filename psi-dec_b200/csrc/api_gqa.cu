@@ -112,8 +112,6 @@ static void reserved_layout(psi_gqa* g) {
     cursor += pad_words(t);
     g->off_token_indices = cursor;
     cursor += pad_words(t);
-    g->off_weigh = cursor;
-    cursor += (t + 2) * kWeighRequestWords;
     g->off.cta = cursor;
     cursor += pad_words(g->grid_cap + 2);
     g->off.first_items = cursor;
@@ -126,6 +124,8 @@ static void reserved_layout(psi_gqa* g) {
     cursor += pad_words(g->cap_chunk_items * kItemWords);
     g->off.reduces = cursor;
     cursor += pad_words(g->cap_reduces * 2);
+    g->off_weigh = cursor;
+    cursor += (t + 2) * kWeighRequestWords;
     g->staging_words = cursor;
 }
 

@@ -206,6 +206,9 @@ struct psi_weigh_plan {
     bool too_large = false;
     bool parted = false;                 // rows of a long run are cut into parts in the second pass
     bool captured = false;               // a captured launch sequence holds key-weight launches
+    bool wanted = false;                 // psi_gqa_weigh_keys has been called: psi_gqa_prepare plans and uploads for it
+    bool planned = false;                // for the prepared batch
+    std::vector<uint32_t> batch_slots, batch_tokens;  // of the prepared batch
     std::vector<uint32_t> seen;          // by slot: the epoch that last named it
     uint32_t epoch = 0;
     psi::DeviceBuffer norms, partials, counters, scores, sums;

@@ -131,6 +131,22 @@ void plan_weigh(psi_gqa* g, const uint32_t* req_slots, const uint32_t* token_ind
 
 namespace {
 
+// The first call on a component: what psi_gqa_prepare does for key weights from then on, for the batch at hand.
+void plan_prepared(psi_gqa* g) {
+    psi_ctx* ctx = g->ctx;
+    psi_weigh_plan& w = g->weigh;
+    plan_weigh(g, w.batch_slots.data(), w.batch_tokens.data(), g->batch_cu.data(), static_cast<uint32_t>(w.batch_slots.size()));
+    const uint32_t counts[2] = {w.num_short, w.num_long};
+    static_assert(kScalarWeighLong == kScalarWeighShort + 1);
+    // pageable sources: staged before the calls return
+    cuda_check(cudaMemcpyAsync(static_cast<uint32_t*>(g->block.ptr) + kScalarWeighShort, counts, sizeof(counts), cudaMemcpyHostToDevice, ctx->stream),
+               "cudaMemcpyAsync");
+    cuda_check(cudaMemcpyAsync(static_cast<uint32_t*>(g->block.ptr) + g->off_weigh, w.reqs.data(), w.reqs.size() * sizeof(WeighRequest),
+                               cudaMemcpyHostToDevice, ctx->stream),
+               "cudaMemcpyAsync");
+    w.wanted = w.planned = true;
+}
+
 uint64_t table_tokens(const psi_gqa* g) {
     return uint64_t(g->cfg.layout.num_blocks) * g->cfg.layout.num_page_ids_per_block * g->tokens_per_page;
 }
@@ -158,6 +174,14 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
         psi_weigh_plan& w = g->weigh;
         require(g->prepared, "GQA batch metadata must be updated before recording");
         require(q != nullptr && weights != nullptr, "q and weights must not be null");
+        const bool fixed = g->replay_reserved;
+        require(!ctx->capturing || fixed, "reserve replay capacity before capturing key-weight launches");
+        ctx->bind();
+        if (!w.planned) {
+            require(!ctx->capturing,
+                    "call psi_gqa_weigh_keys once after the replay reservation and before the capture: it allocates its scratch then");
+            plan_prepared(g);
+        }
         require(!w.repeated, "a request slot appears twice in the batch: its keys cannot gather weight from two requests at once");
         require(!w.too_large, "the batch exceeds the key-weight kernels' work counts");
         WeighParams p{};
@@ -168,11 +192,8 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
         require((reinterpret_cast<uintptr_t>(weights) & 3u) == 0, "weights must be 4-byte aligned");
         require(reinterpret_cast<uintptr_t>(q) % dtype_bytes(g->cfg.dtype) == 0, "q must be aligned to its elements");
         require(weights_stride >= w.max_keys, "the weights' row stride must hold every key of the batch");
-        const bool fixed = g->replay_reserved;
-        require(!ctx->capturing || fixed, "reserve replay capacity before capturing key-weight launches");
         require(!ctx->capturing || weights_stride >= table_tokens(g),
                 "captured key-weight launches need rows of weights as long as the page table's");
-        ctx->bind();
         const uint32_t heads = g->cfg.num_kv_heads, group = g->cfg.num_q_heads / heads;
         const uint64_t sms = static_cast<uint64_t>(ctx->sm_count);
         const uint32_t block = tensor ? kWeighBlock : kWeighAnyRows;
