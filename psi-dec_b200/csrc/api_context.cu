@@ -154,6 +154,7 @@ int32_t psi_ctx_capture_begin(psi_ctx* ctx) {
         ctx->bind();
         cuda_check(cudaStreamBeginCapture(ctx->stream, cudaStreamCaptureModeThreadLocal), "cudaStreamBeginCapture");
         ctx->capturing = true;
+        ctx->capture_marks.clear();
     });
 }
 
@@ -164,11 +165,14 @@ int32_t psi_ctx_capture_end(psi_ctx* ctx, psi_graph** out) {
         *out = nullptr;
         require(ctx->capturing, "no stream capture is open on this context");
         ctx->capturing = false;
+        const std::vector<std::shared_ptr<int>> marks = std::move(ctx->capture_marks);
+        ctx->capture_marks.clear();
         cudaGraph_t graph = nullptr;
         cuda_check(cudaStreamEndCapture(ctx->stream, &graph), "cudaStreamEndCapture");
         auto holder = std::make_unique<psi_graph>();
         holder->ctx = ctx;
         holder->graph = graph;
+        holder->marks = marks;
         size_t nodes = 0;
         cuda_check(cudaGraphGetNodes(graph, nullptr, &nodes), "cudaGraphGetNodes");
         std::vector<cudaGraphNode_t> list(nodes);

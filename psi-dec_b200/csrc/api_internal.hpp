@@ -51,6 +51,7 @@ struct psi_ctx {
     std::string last_error;
     bool timing = false;
     bool capturing = false;  // between psi_ctx_capture_begin and psi_ctx_capture_end
+    std::vector<std::shared_ptr<int>> capture_marks;  // the open capture's, for its graph
     // (begin, end) event pairs per kernel class, recorded while timing is on
     std::vector<std::pair<cudaEvent_t, cudaEvent_t>> timed[psi::kKernelClasses];
     void bind() const { psi::cuda_check(cudaSetDevice(device), "cudaSetDevice"); }
@@ -163,6 +164,7 @@ struct psi_graph {
     cudaGraph_t graph = nullptr;
     cudaGraphExec_t exec = nullptr;
     uint64_t kernel_nodes = 0;
+    std::vector<std::shared_ptr<int>> marks;  // of components that have to know while the graph lives
 };
 
 struct psi_snapshot_writer {
@@ -205,7 +207,7 @@ struct psi_weigh_plan {
     bool repeated = false;               // a slot appears twice in the batch
     bool too_large = false;
     bool parted = false;                 // rows of a long run are cut into parts in the second pass
-    bool captured = false;               // a captured launch sequence holds key-weight launches
+    std::weak_ptr<int> captured;         // lives while a captured launch sequence holds key-weight launches
     bool wanted = false;                 // psi_gqa_weigh_keys has been called: psi_gqa_prepare plans and uploads for it
     bool planned = false;                // for the prepared batch
     std::vector<uint32_t> batch_slots, batch_tokens;  // of the prepared batch

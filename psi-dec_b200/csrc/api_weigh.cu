@@ -123,7 +123,7 @@ void plan_weigh(psi_gqa* g, const uint32_t* req_slots, const uint32_t* token_ind
     w.span_keys = tensor ? w.reqs.back().first_pos * kWeighBlock : kWeighAnyKeys;
     w.stats_items = cu0;
     w.sum_items = cu1;
-    require(!w.captured || (!w.repeated && !w.too_large),
+    require(w.captured.expired() || (!w.repeated && !w.too_large),
             "a request slot appears twice in the batch: the captured key-weight launches cannot add to its keys twice at once");
 }
 
@@ -264,7 +264,11 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
             }
             p.scores = static_cast<float*>(w.scores.ptr);
         }
-        if (ctx->capturing) w.captured = true;
+        if (ctx->capturing) {
+            std::shared_ptr<int> mark = w.captured.lock();
+            if (mark == nullptr) w.captured = mark = std::make_shared<int>(0);
+            ctx->capture_marks.push_back(std::move(mark));
+        }
         if (short_ctas > 0) run_pass(g, p, keep_scores ? WeighPass::kShortStatsScores : WeighPass::kShortStats, short_ctas);
         const uint64_t long_wave = tensor ? sms : sms * (g->cfg.head_dim > 96 ? 2 : 4);
         const uint64_t stats_ctas = fixed ? (can_long ? long_wave : 0) : std::min<uint64_t>(long_wave, w.stats_items);
