@@ -600,8 +600,9 @@ PSI_API int32_t psi_gqa_attend_static(int32_t device, void* cuda_stream, const p
  * finite maximum adds nothing.  Sums are f32 in a fixed order: the same call gives the same bits.
  * 16-bit profiles whose head_dim is a multiple of eight run on the tensor cores and need q and the arena on 16-byte boundaries;
  * every other profile of the component runs on the CUDA cores.  A batch that names a slot twice is refused.
- * Scratch is allocated on the first call and grows with the batch (4 bytes per query row and key of the short runs, up to
- * 2 GiB; without it the keys are read twice).  In a captured sequence (after psi_gqa_reserve_replay and one call outside the
+ * Scratch is allocated on the first call and grows by half with the batch, which waits for the stream: 4 bytes for each key and KV
+ * head of the short runs (16 query rows of a KV head or fewer) and row of the longest among them, up to 2 GiB; where that is not
+ * enough, or the device has no room for it, their keys are read twice instead.  In a captured sequence (after psi_gqa_reserve_replay and one call outside the
  * capture) weights_stride must hold the page table's whole row, and while a graph of such a capture lives psi_gqa_prepare
  * refuses a batch that names a slot twice, for which the replay would add to one row from two requests at once. */
 PSI_API int32_t psi_gqa_weigh_keys(psi_gqa* gqa, psi_pages* pages, psi_table* table, uint32_t layer, const void* q, float* weights,

@@ -117,6 +117,23 @@ struct DeviceBuffer {
         bytes = wanted;
         if (zero) cuda_check(cudaMemsetAsync(ptr, 0, wanted, ctx->stream), "cudaMemsetAsync");
     }
+    // Another buffer of `wanted` bytes instead of this one, which stays where there is no room for both.
+    bool replace(psi_ctx* ctx, uint64_t wanted) {
+        require(!ctx->capturing, "a device buffer would have to grow during stream capture: reserve replay capacity first");
+        void* fresh = nullptr;
+        const cudaError_t err = cudaMalloc(&fresh, wanted);
+        if (err == cudaErrorMemoryAllocation) {
+            (void)cudaGetLastError();
+            return false;
+        }
+        cuda_check(err, "cudaMalloc");
+        const cudaError_t waited = ptr == nullptr ? cudaSuccess : cudaStreamSynchronize(ctx->stream);
+        release();
+        ptr = fresh;
+        bytes = wanted;
+        cuda_check(waited, "cudaStreamSynchronize");
+        return true;
+    }
     void release() {
         if (ptr != nullptr) (void)cudaFree(ptr);
         ptr = nullptr;
@@ -214,6 +231,7 @@ struct psi_weigh_plan {
     std::vector<uint32_t> seen;          // by slot: the epoch that last named it
     uint32_t epoch = 0;
     psi::DeviceBuffer norms, partials, counters, scores, sums;
+    uint64_t scores_refused = UINT64_MAX;  // a size of `scores` that could not be had
 };
 
 struct psi_gqa {

@@ -151,6 +151,8 @@ uint64_t table_tokens(const psi_gqa* g) {
     return uint64_t(g->cfg.layout.num_blocks) * g->cfg.layout.num_page_ids_per_block * g->tokens_per_page;
 }
 
+constexpr uint64_t kMostScratch = 2ull << 30;
+
 void run_pass(psi_gqa* g, const WeighParams& p, WeighPass pass, uint64_t ctas) {
     LaunchScope scope(g->ctx, PSI_KERNEL_CLASS_WEIGH);
     cuda_check(launch_weigh(p, pass, static_cast<uint32_t>(ctas), g->ctx->stream), "key weight launch");
@@ -218,11 +220,12 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
             require(w.norms.ptr != nullptr && partial_bytes <= w.partials.bytes && counter_words * sizeof(uint32_t) <= w.counters.bytes,
                     "call psi_gqa_weigh_keys once after the replay reservation and before the capture: it allocates its scratch then");
         } else {
-            require(!fixed || partial_bytes <= (2ull << 30),
+            require(!fixed || partial_bytes <= kMostScratch,
                     "the replay reservation needs more than 2 GiB of key-weight scratch for this max_tokens: create the component with "
                     "the largest batch the replayed steps carry");
             w.norms.ensure(ctx, uint64_t(g->cfg.max_tokens) * g->cfg.num_q_heads * sizeof(float2), false);
-            w.partials.ensure(ctx, partial_bytes > w.partials.bytes ? std::max<uint64_t>(partial_bytes * 3 / 2, 1 << 16) : partial_bytes, false);
+            // (the reservation's size is the last one)
+            w.partials.ensure(ctx, partial_bytes <= w.partials.bytes || fixed ? partial_bytes : std::max<uint64_t>(partial_bytes * 3 / 2, 1 << 16), false);
             w.sums.ensure(ctx, sum_bytes > w.sums.bytes ? sum_bytes * 3 / 2 : sum_bytes, false);
             if (counter_words * sizeof(uint32_t) > w.counters.bytes) {
                 w.counters.release_after(ctx);  // counters restart from zero at their new size
@@ -254,14 +257,7 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
             // the second pass reads the keys again instead (32 requests of 1,024 to 8,192 keys, 2 KV heads x 256, 8 rows: 51 us with
             // scratch, 73 without).
             const uint64_t bytes = w.tiles * kWeighTile * p.score_rows * sizeof(float);
-            keep_scores = bytes <= (2ull << 30);
-            if (keep_scores && bytes > w.scores.bytes) {
-                try {
-                    w.scores.ensure(ctx, bytes + bytes / 2, false);
-                } catch (const ExhaustedError&) {
-                    keep_scores = false;
-                }
-            }
+            keep_scores = grow_scratch(bytes, w.scores.bytes, kMostScratch, w.scores_refused, [&](uint64_t wanted) { return w.scores.replace(ctx, wanted); });
             p.scores = static_cast<float*>(w.scores.ptr);
         }
         if (ctx->capturing) {

@@ -36,6 +36,20 @@ constexpr uint32_t kMaxRows = 16;   // query rows (tokens x heads) one work item
 
 inline uint32_t dtype_bytes(uint32_t dtype) { return dtype == PSI_DTYPE_F32 ? 4u : 2u; }
 
+// Scratch that a call can do without.  Grows by half, up to `limit`, or where that cannot be had to what is asked for; a size that
+// could not be had is not asked for again.  allocate(bytes) replaces the buffer of `have` bytes, or leaves it and returns false.
+template <typename Allocate>
+bool grow_scratch(uint64_t wanted, uint64_t have, uint64_t limit, uint64_t& refused, const Allocate& allocate) {
+    if (wanted > limit) return false;
+    if (wanted <= have) return true;
+    if (wanted >= refused) return false;
+    const uint64_t half_more = wanted + wanted / 2, roomy = half_more < limit ? half_more : limit;
+    if (roomy < refused && roomy > wanted && allocate(roomy)) return true;
+    if (allocate(wanted)) return true;
+    refused = wanted;
+    return false;
+}
+
 // ---- replay buckets (crates/inference-executor-core/src/replay.rs) ------------------------------------------------
 class BucketPolicy {
 public:
