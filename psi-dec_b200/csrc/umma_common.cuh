@@ -172,7 +172,7 @@ __device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
     return v;
 }
 
-__device__ __forceinline__ float fast_exp2(float x) {
+__device__ __forceinline__ float fast_exp2(float x) {  // 2 ulp; results below the smallest normal number are 0
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;

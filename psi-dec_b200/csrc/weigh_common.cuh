@@ -2,17 +2,12 @@
 #pragma once
 
 #include "mma_common.cuh"
+#include "umma_common.cuh"
 #include "weigh_keys.hpp"
 
 namespace psi {
 
 constexpr float kInf = INFINITY;
-
-__device__ __forceinline__ float exp2_approx(float x) {  // 2 ulp; results below the smallest normal number are 0
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 // The request whose work holds `index`: the last one whose prefix (`which` 0: cu0, 1: cu1) is at or below it.  By a converged warp,
 // 32 requests at a time: a search that halves would wait for a load in each of its steps.
@@ -47,7 +42,7 @@ struct Stat {
 
 // The weight of a key from its product with the query row.
 __device__ __forceinline__ float weight_of(float product, float scale_log2, float2 norm) {
-    return norm.y > 0.0f ? exp2_approx(fmaf(product, scale_log2, -norm.x)) * norm.y : 0.0f;
+    return norm.y > 0.0f ? fast_exp2(fmaf(product, scale_log2, -norm.x)) * norm.y : 0.0f;
 }
 
 // Query row r of a request and KV head as (flat token, head) row of q.
@@ -58,13 +53,6 @@ __device__ __forceinline__ uint64_t query_row(const WeighParams& p, const WeighR
 // Keys that row r sees.
 __device__ __forceinline__ uint32_t row_limit(const WeighParams& p, const WeighRequest& rq, uint32_t r) {
     return rq.first_pos + r / p.group + 1;
-}
-
-__device__ __forceinline__ const uint4* key_row(const WeighParams& p, const PageBounds& bounds, const uint32_t* row_ids,
-                                                uint32_t head, uint32_t key, uint32_t& bad) {
-    const uint32_t page = bounds.read(row_ids, key / p.geo.tokens_per_page, bad);
-    const uint64_t at = kv_row_offset(p.geo, page, head, key % p.geo.tokens_per_page);
-    return reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.geo.pages) + at);
 }
 
 __device__ __forceinline__ float* weight_row(const WeighParams& p, const WeighRequest& rq, uint32_t head) {

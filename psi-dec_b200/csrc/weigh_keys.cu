@@ -220,19 +220,19 @@ __global__ __launch_bounds__(256, 1) void weigh_short_kernel(const WeighParams p
                     }
                     const float m0 = fmaxf(s0.m, fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])) * p.scale_log2);
                     const float base0 = m0 == -kInf ? 0.0f : m0;
-                    s0.l *= exp2_approx(s0.m - base0);
+                    s0.l *= fast_exp2(s0.m - base0);
                     s0.m = m0;
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
-                        s0.l += exp2_approx(fmaf(s[t][0], p.scale_log2, -base0)) + exp2_approx(fmaf(s[t][1], p.scale_log2, -base0));
+                        s0.l += fast_exp2(fmaf(s[t][0], p.scale_log2, -base0)) + fast_exp2(fmaf(s[t][1], p.scale_log2, -base0));
                     if (two_halves) {
                         const float m1 = fmaxf(s1.m, fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])) * p.scale_log2);
                         const float base1 = m1 == -kInf ? 0.0f : m1;
-                        s1.l *= exp2_approx(s1.m - base1);
+                        s1.l *= fast_exp2(s1.m - base1);
                         s1.m = m1;
 #pragma unroll
                         for (int t = 0; t < 2; ++t)
-                            s1.l += exp2_approx(fmaf(s[t][2], p.scale_log2, -base1)) + exp2_approx(fmaf(s[t][3], p.scale_log2, -base1));
+                            s1.l += fast_exp2(fmaf(s[t][2], p.scale_log2, -base1)) + fast_exp2(fmaf(s[t][3], p.scale_log2, -base1));
                     }
                 }
             }
@@ -464,10 +464,10 @@ __global__ __launch_bounds__(kAnyThreads) void weigh_stats_any_kernel(const Weig
                 }
                 m = fmaxf(st[a].m, m * p.scale_log2);
                 const float base = m == -kInf ? 0.0f : m;
-                st[a].l *= exp2_approx(st[a].m - base);
+                st[a].l *= fast_exp2(st[a].m - base);
                 st[a].m = m;
 #pragma unroll
-                for (int b = 0; b < 4; ++b) st[a].l += exp2_approx(fmaf(s[a][b], p.scale_log2, -base));
+                for (int b = 0; b < 4; ++b) st[a].l += fast_exp2(fmaf(s[a][b], p.scale_log2, -base));
             }
             __syncthreads();
         }

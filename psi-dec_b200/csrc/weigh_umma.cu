@@ -186,14 +186,14 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_umma_kernel(const WeighPara
                     float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
                     top = max3_nan(st.m, st.m, top * p.scale_log2);
                     const float base = top == -kInf ? 0.0f : top;
-                    st.l *= exp2_approx(st.m - base);
+                    st.l *= fast_exp2(st.m - base);
                     st.m = top;
                     const uint64_t base2 = pack_f32x2(-base, -base);
                     uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
                     for (uint32_t c = 0; c < kColumns; c += 2) {
                         const float2 x = unpack_f32x2(fma_f32x2(pack_f32x2(s[c], s[c + 1]), scale2, base2));
-                        sum[c >> 1 & 3] = add_f32x2(sum[c >> 1 & 3], pack_f32x2(exp2_approx(x.x), exp2_approx(x.y)));
+                        sum[c >> 1 & 3] = add_f32x2(sum[c >> 1 & 3], pack_f32x2(fast_exp2(x.x), fast_exp2(x.y)));
                     }
                     const float2 all = unpack_f32x2(add_f32x2(add_f32x2(sum[0], sum[1]), add_f32x2(sum[2], sum[3])));
                     st.l += all.x + all.y;
@@ -256,8 +256,8 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_umma_kernel(const WeighPara
                                 const ulonglong2 inverse = *reinterpret_cast<const ulonglong2*>(&numbers.inverse[column0 + c]);
                                 float2 x = unpack_f32x2(fma_f32x2(pack_f32x2(s[c], s[c + 1]), scale2, base.x));
                                 float2 y = unpack_f32x2(fma_f32x2(pack_f32x2(s[c + 2], s[c + 3]), scale2, base.y));
-                                x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-                                y = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+                                x = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+                                y = make_float2(fast_exp2(y.x), fast_exp2(y.y));
                                 if constexpr (decltype(with_mask)::value) {
                                     const uint4 limit = *reinterpret_cast<const uint4*>(&numbers.limit[column0 + c]);
                                     const float2 i0 = unpack_f32x2(inverse.x), i1 = unpack_f32x2(inverse.y);
