@@ -12,7 +12,8 @@ struct psi_linear {
     cudaEvent_t upload_done = nullptr;
     DeviceBuffer decays;       // [layers][Hv][kLinearDecays]
     DeviceBuffer status_word;  // u32 written by bounded device-side waits
-    bool chunked = false;      // long runs take the chunked form
+    bool chunked = false;      // long runs take the chunked form,
+    uint32_t step_tokens = 0;  // those of more tokens than this
     DeviceBuffer carries;      // [max_carries][Hv][Dk][Dv]: states between the pieces of a request
     uint32_t max_carries = 0;
     uint32_t num_steps = 0, num_runs = 0, num_carries = 0, num_scans = 0, num_tokens = 0;  // of the prepared batch
@@ -22,9 +23,12 @@ struct psi_linear {
 
 namespace {
 
-// Runs of more tokens take the chunked form, which costs the same from 1 to 64 tokens.  16/32 heads x 128, bf16, recurrent and chunked:
-// 9 tokens 20 and 21 us, 16 tokens 22 and 20; 32 requests of 9 tokens 65 and 65 us, of 12 tokens 82 and 66, of 16 tokens 95 and 67.
-constexpr uint32_t kStepTokens = 8;
+// Runs of more tokens take the chunked form, which costs the same from 1 to 64 tokens; the recurrent form's cost grows with the tokens
+// and the state.  16/32 heads, bf16, launches one behind the other, recurrent and chunked in us, for one request, 32 and 128:
+//   128 x 128, 9 tokens    6.2 and 8.7,  49 and 53,  191 and 227        64 x 64, 16 tokens   5.5 and 6.0,  25 and 33,   88 and 132
+//   10 tokens              7.1 and 8.7,  58 and 53,  225 and 228        24 tokens            7.1 and 6.1,  34 and 33,  125 and 133
+//   16 tokens              8.3 and 8.7,  77 and 54,  300 and 228
+uint32_t step_tokens(const psi_linear_config& c) { return c.key_dim <= 64 && c.value_dim <= 64 ? 16 : 9; }
 
 // Into how many chunks the pieces of a batch's long runs are cut (0: nothing is cut).  The chunked form takes one CTA per run and head
 // through its chunks in turn, so that few heads leave SMs idle; pieces side by side cost a pass for the states between them.  In units
@@ -110,7 +114,8 @@ int32_t psi_linear_create(psi_ctx* ctx, const psi_linear_config* config, psi_lin
         for (uint64_t i = 0; i < decays; ++i) fill_decay(none.data() + i * kLinearDecays, 0.0f);
         // pieces for four rounds of CTAs
         l->max_carries = std::max<uint32_t>(2, 4 * static_cast<uint32_t>(ctx->sm_count) / c.num_v_heads);
-        l->chunked = linear_chunk_supported(c.dtype, c.key_dim, c.value_dim) && c.max_tokens > kStepTokens;
+        l->step_tokens = step_tokens(c);
+        l->chunked = linear_chunk_supported(c.dtype, c.key_dim, c.value_dim) && c.max_tokens > l->step_tokens;
         try {
             l->block.ensure(ctx, block_capacity(l.get()) * sizeof(uint32_t), true);
             l->status_word.ensure(ctx, sizeof(uint32_t), true);
@@ -207,14 +212,14 @@ int32_t psi_linear_prepare(psi_linear* l, const uint32_t* req_slots, const uint3
         uint32_t n = 0;
         for (uint32_t r = 0; r < num_reqs; ++r) {
             const uint32_t q_len = cu_tokens[r + 1] - cu_tokens[r];
-            if (q_len > 0 && !(l->chunked && q_len > kStepTokens))
+            if (q_len > 0 && !(l->chunked && q_len > l->step_tokens))
                 reqs[n++] = LinearRequest{req_slots[r], outs[r], token_indices[r] == 0 ? 1u : 0u, q_len, cu_tokens[r], {0, 0, 0}};
         }
         l->num_steps = n;
         // the long runs in pieces: those that another one follows first, then the ends
         std::vector<uint32_t> long_runs, run_tokens;
         for (uint32_t r = 0; r < num_reqs && l->chunked; ++r) {
-            if (cu_tokens[r + 1] - cu_tokens[r] <= kStepTokens) continue;
+            if (cu_tokens[r + 1] - cu_tokens[r] <= l->step_tokens) continue;
             long_runs.push_back(r);
             run_tokens.push_back(cu_tokens[r + 1] - cu_tokens[r]);
         }
