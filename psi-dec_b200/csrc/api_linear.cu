@@ -32,9 +32,9 @@ uint32_t step_tokens(const psi_linear_config& c) { return c.key_dim <= 64 && c.v
 
 // Into how many chunks the pieces of a batch's long runs are cut (0: nothing is cut).  The chunked form takes one CTA per run and head
 // through its chunks in turn, so that few heads leave SMs idle; pieces side by side cost a pass for the states between them.  In units
-// of a chunk's time (2.0 us at 128 x 128, the state pass's 0.5 of it): a launch takes the longest CTA's chunks, the CTAs going round
-// their items, and the scan with its two launches three.  128 x 128, cut and whole: 32 heads, 1,024 tokens 39 and 46 us, 8,192 tokens
-// 139 and 251; 4 heads, 512 tokens 30 and 29, 1,024 tokens 31 and 45, 8,192 tokens 46 and 249.
+// of a chunk's time (2.2 us at 128 x 128 in bf16, the state pass's 0.5 of it): a launch takes the longest CTA's chunks, the CTAs going
+// round their items, and the scan with its two launches three.  128 x 128, bf16, cut and whole: 32 heads, 1,024 tokens 38 and 46 us,
+// 8,192 tokens 157 and 284; 4 heads, 512 tokens 26 and 28, 1,024 tokens 28 and 45, 8,192 tokens 46 and 278.
 uint32_t piece_chunks(const std::vector<uint32_t>& run_tokens, uint32_t heads, uint32_t sms, uint32_t max_carries) {
     uint32_t longest = 0;
     const auto chunks_of = [](uint32_t tokens) { return (tokens + kLinearChunk - 1) / kLinearChunk; };

@@ -15,8 +15,8 @@
 //                                              others in TMEM), f16 two (22 bits)
 //
 // Every part is a product of its own into the same accumulator, the lowest part first; in f16 the low part is held 2^11 times as large.
-// Two parts of P and S make 16 bits in bf16 and 22 in f16, so that an output is off by its own rounding (one part alone: 1.4 times that;
-// 8,192 tokens 142 us for 158).  In f16 each row of P and each column of S is scaled by a power of two first, so that
+// Two parts of P and S, the first towards zero, are off by 2^-15 of a value in bf16 and 2^-21 in f16, so that an output is off by its own
+// rounding (one part alone: 1.4 times that; 8,192 tokens 142 us for 154).  In f16 each row of P and each column of S is scaled by a power of two first, so that
 // nothing leaves f16's range; the weighted V is not scaled: below 2^-14 its parts have an absolute step of 2^-35, so that
 // a state which only such values make has fewer bits than 22.  The state itself stays in f32 registers; a chunk's gain is
 // added to it after an accumulation of its own, since the tensor cores' accumulation truncates.
@@ -28,9 +28,9 @@
 // is off its 16-byte boundaries; rows that the last box brings from behind a run are cleared by the state threads) and issues
 // the gains, the longest chain from chunk to chunk, which wait for the state threads alone.  The loops are kept short: unrolled, the
 // roles' code together ran out of the instruction cache and took 1.5 times as long.
-// Bound by the chain of one head's chunks, 4,000 cycles each at 128 x 128, of which the state threads work for nearly all; the
-// products are 1,500.  One prompt of 8,192 tokens, 32 heads, f16: 158 us in pieces (42 of bytes, 10 of
-// products); three prompts of 926 to 2,185 tokens, 16/32 heads, bf16: 83 us.
+// Bound by the chain of one head's chunks at 128 x 128, 2.2 us each in bf16 and 2.6 in f16, of which the state threads work for
+// nearly all (without the second parts' products it is as long, without their arithmetic 6 % shorter).  One prompt of 8,192 tokens, 32
+// heads, f16: 154 us in pieces (42 of bytes, 10 of products), 337 whole; three prompts of 926 to 2,185 tokens, 16/32 heads, bf16: 83 us.
 // Every hand-off is an mbarrier, every wait is bounded and reports PSI_ERR_TIMEOUT through the status word, and TMEM is freed on
 // every path.
 #include <cstddef>
@@ -116,13 +116,15 @@ __device__ __forceinline__ void split_parts(uint64_t x, uint32_t (&part)[3]) {
     }
 }
 
-// The same in two parts: bf16 the first towards zero, f16 the second 2^11 times as large.
+// The same in two parts, the first towards zero: f16 by its leading bits, without a conversion back.  (A value below f16's normal range,
+// 2^-24 of the largest beside it and less, loses what its first part rounds.)
 template <typename T>
 __device__ __forceinline__ void split_two(uint64_t x, uint32_t& high, uint32_t& low) {
     float2 v = unpack_f32x2(x);
     if constexpr (kIsHalf<T>) {
-        high = Mma<T>::pack(v.x, v.y);
-        v = unpack_f32x2(mul_f32x2(rest_of(x, Mma<T>::unpack(high)), pack_f32x2(2048.0f, 2048.0f)));
+        const float2 lead = make_float2(__uint_as_float(__float_as_uint(v.x) & 0xFFFFE000u), __uint_as_float(__float_as_uint(v.y) & 0xFFFFE000u));
+        high = Mma<T>::pack(lead.x, lead.y);
+        v = unpack_f32x2(mul_f32x2(rest_of(x, lead), pack_f32x2(2048.0f, 2048.0f)));
     } else {
         high = Mma<T>::pack_down(v.x, v.y);
         v = unpack_f32x2(rest_of(x, Mma<T>::unpack(high)));
