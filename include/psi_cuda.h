@@ -600,6 +600,9 @@ PSI_API int32_t psi_gqa_attend_static(int32_t device, void* cuda_stream, const p
  * finite maximum adds nothing.  Sums are f32 in a fixed order: the same call gives the same bits.
  * 16-bit profiles whose head_dim is a multiple of eight run on the tensor cores and need q and the arena on 16-byte boundaries;
  * every other profile of the component runs on the CUDA cores.  A batch that names a slot twice is refused.
+ * The softmax is over the keys that the batch names on this device.  Where a context is split over devices (psi_gqa_attend_partial,
+ * psi_gqa_attend_exchange), each shard's call sums weights of its own keys alone, which are not the context's and do not compare
+ * between shards: cut such a context on one device, or not by these weights.
  * Scratch is allocated on the first call and grows by half with the batch, which waits for the stream: 4 bytes for each key and KV
  * head of the short runs (16 query rows of a KV head or fewer) and row of the longest among them, up to 2 GiB; where that is not
  * enough, or the device has no room for it, their keys are read twice instead.  In a captured sequence (after psi_gqa_reserve_replay and one call outside the
@@ -655,7 +658,8 @@ PSI_API int32_t psi_linear_prepare(psi_linear* linear, const uint32_t* req_slots
 /* q, k device [T][Hk][key_dim], v, out device [T][Hv][value_dim]; out must not overlap the inputs.  Any number of tokens per
  * request.  The same call gives the same bits.  May be captured: a replay takes the batch prepared last, and the buffers of a
  * captured call hold max_tokens rows, whatever batch comes (rows behind the batch are read over and not used).  A token whose
- * q, k or v is not finite reaches no token before it and no other request. */
+ * q, k or v is not finite reaches no token before it and no other request; what the formulas make infinite from it on may come out
+ * as NaN. */
 PSI_API int32_t psi_linear_attend(psi_linear* linear, uint32_t layer, float* states, const void* q, const void* k, const void* v,
                                   void* out);
 /* As psi_gqa_device_status: waits for the stream; PSI_ERR_TIMEOUT when a bounded wait of a launch gave up. */

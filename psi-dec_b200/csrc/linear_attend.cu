@@ -2,6 +2,8 @@
 //
 //   S_t = lambda S_{t-1} + k_t^T v_t        o_t = scale q_t S_t        S: f32 [Dk][Dv]
 //
+// (A state that is not finite stays so, as NaN after another token: the decay's low part is 0 or of the other sign.  So may its
+// outputs: the rows that pad key_dim to the compiled count hold 0 v.)
 // linear_step_kernel, the recurrent form: a CTA takes 32 columns of one head's state of one request into registers, goes through
 // the request's tokens and writes the columns back: bound by the state's bytes, read and written once for the whole run.  A
 // decay close to one that is rounded to f32 would be off by up to 2^-25 a token, and all in the same direction; it is held as two f32
