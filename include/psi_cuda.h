@@ -605,8 +605,8 @@ PSI_API int32_t psi_gqa_attend_static(int32_t device, void* cuda_stream, const p
  * between shards: cut such a context on one device, or not by these weights.
  * Scratch is allocated on the first call and grows by half with the batch, which waits for the stream: 4 bytes for each key and KV
  * head of the short runs (16 query rows of a KV head or fewer) and row of the longest among them, up to 2 GiB; where that is not
- * enough, or the device has no room for it, their keys are read twice instead.  In a captured sequence (after psi_gqa_reserve_replay and one call outside the
- * capture) weights_stride must hold the page table's whole row, and while a graph of such a capture lives psi_gqa_prepare
+ * enough, or the device has no room for it, their keys are read twice instead.  In a sequence captured by psi_ctx_capture_begin (after
+ * psi_gqa_reserve_replay and one call outside the capture; a capture of the host's own is refused) weights_stride must hold the page table's whole row, and while a graph of such a capture lives psi_gqa_prepare
  * refuses a batch that names a slot twice, for which the replay would add to one row from two requests at once. */
 PSI_API int32_t psi_gqa_weigh_keys(psi_gqa* gqa, psi_pages* pages, psi_table* table, uint32_t layer, const void* q, float* weights,
                                    uint64_t weights_stride);
@@ -656,7 +656,7 @@ PSI_API int32_t psi_linear_set_decay(psi_linear* linear, uint32_t layer, const f
 PSI_API int32_t psi_linear_prepare(psi_linear* linear, const uint32_t* req_slots, const uint32_t* out_slots,
                                    const uint32_t* token_indices, const uint32_t* cu_tokens, uint32_t num_reqs);
 /* q, k device [T][Hk][key_dim], v, out device [T][Hv][value_dim]; out must not overlap the inputs.  Any number of tokens per
- * request.  The same call gives the same bits.  May be captured: a replay takes the batch prepared last, and the buffers of a
+ * request.  The same call gives the same bits.  May be captured, by psi_ctx_capture_begin or by the host itself: a replay takes the batch prepared last, and the buffers of a
  * captured call hold max_tokens rows, whatever batch comes (rows behind the batch are read over and not used).  A token whose
  * q, k or v is not finite reaches no token before it and no other request; what the formulas make infinite from it on may come out
  * as NaN. */

@@ -328,7 +328,7 @@ int32_t psi_gqa_set_positions(psi_gqa* g, const uint32_t* positions, uint32_t nu
         psi_ctx* ctx = g->ctx;
         require(g->prepared, "GQA batch metadata must be updated before its positions");
         require(g->has_norm_rope, "psi_gqa_set_norm_rope must be called before psi_gqa_set_positions");
-        require(!ctx->capturing, "psi_gqa_set_positions uploads the step's positions and stays outside captured graphs");
+        require(!stream_captured(ctx), "psi_gqa_set_positions uploads the step's positions and stays outside captured graphs");
         require(positions != nullptr, "positions must not be null");
         const std::vector<uint32_t>& cu = g->batch_cu;
         require(num_reqs + 1ull == cu.size(), "positions must name every request of the prepared batch");

@@ -68,6 +68,15 @@ struct psi_ctx {
 
 namespace psi {
 
+// The context's stream is being captured, by psi_ctx_capture_begin or by the host itself.
+inline bool stream_captured(const psi_ctx* ctx) {
+    if (ctx->capturing) return true;
+    if (ctx->stream == nullptr || ctx->stream == cudaStreamLegacy) return false;  // never captured
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    cuda_check(cudaStreamIsCapturing(ctx->stream, &status), "cudaStreamIsCapturing");
+    return status != cudaStreamCaptureStatusNone;
+}
+
 // Counts one launch, names it for a timeline profiler (an NVTX range per launch: a no-op costing a few nanoseconds
 // when no tool is attached), and, while timing is on, brackets it with events on the context's stream.
 struct LaunchScope {

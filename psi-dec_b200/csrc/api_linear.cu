@@ -102,7 +102,7 @@ int32_t psi_linear_create(psi_ctx* ctx, const psi_linear_config* config, psi_lin
         require(c.dtype <= PSI_DTYPE_F16, "unsupported linear attention dtype");
         require(c.num_req_slots > 0 && c.num_layers > 0 && c.max_tokens > 0, "linear attention slots, layers and tokens must be positive");
         require(uint64_t(c.max_tokens) * c.num_v_heads * 8 <= kU32Max, "linear attention batch exceeds the kernels' work counts");
-        require(!ctx->capturing, "a linear attention component cannot be created during stream capture");
+        require(!stream_captured(ctx), "a linear attention component cannot be created during stream capture");
         ctx->bind();
         auto l = std::make_unique<psi_linear>();
         l->ctx = ctx;
@@ -160,7 +160,7 @@ int32_t psi_linear_set_decay(psi_linear* l, uint32_t layer, const float* log_dec
         psi_ctx* ctx = l->ctx;
         require(log_decay != nullptr, "log_decay must not be null");
         require(layer < l->cfg.num_layers, "linear attention layer out of range");
-        require(!ctx->capturing, "psi_linear_set_decay uploads the decays and stays outside captured graphs");
+        require(!stream_captured(ctx), "psi_linear_set_decay uploads the decays and stays outside captured graphs");
         const uint32_t heads = l->cfg.num_v_heads;
         std::vector<float> parts(uint64_t(heads) * kLinearDecays);
         for (uint32_t h = 0; h < heads; ++h) {
@@ -179,7 +179,7 @@ int32_t psi_linear_prepare(psi_linear* l, const uint32_t* req_slots, const uint3
     if (l == nullptr) return PSI_ERR_INVALID_ARGUMENT;
     return guarded(l->ctx, [&] {
         psi_ctx* ctx = l->ctx;
-        require(!ctx->capturing, "psi_linear_prepare uploads the step's batch and stays outside captured graphs");
+        require(!stream_captured(ctx), "psi_linear_prepare uploads the step's batch and stays outside captured graphs");
         require(req_slots != nullptr && token_indices != nullptr && cu_tokens != nullptr, "metadata inputs must not be null");
         require(num_reqs > 0, "linear attention batch requires tokens");
         require(cu_tokens[0] == 0, "linear attention batch cu_tokens must start at zero");
@@ -294,18 +294,18 @@ int32_t psi_linear_attend(psi_linear* l, uint32_t layer, float* states, const vo
         p.value_dim = l->cfg.value_dim;
         p.dtype = l->cfg.dtype;
         p.scale = l->cfg.scale;
-        p.num_tokens = ctx->capturing ? l->cfg.max_tokens : l->num_tokens;
+        // a captured launch has to be right for every later batch: its grid and its maps do not depend on this one
+        const bool fixed = stream_captured(ctx);
+        p.num_tokens = fixed ? l->cfg.max_tokens : l->num_tokens;
         p.aligned = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0 ? 1u : 0u;
         const uint64_t wave = static_cast<uint64_t>(ctx->sm_count) * linear_step_resident(l->cfg.key_dim);
         const uint64_t per_request = uint64_t(l->cfg.num_v_heads) * linear_step_slices(l->cfg.value_dim);
-        // a captured launch has to be right for every later batch: its grid does not depend on this one
-        const uint64_t items = (ctx->capturing ? uint64_t(l->cfg.max_tokens) : l->num_steps) * per_request;
+        const uint64_t items = (fixed ? uint64_t(l->cfg.max_tokens) : l->num_steps) * per_request;
         if (items > 0) {
             LaunchScope scope(ctx, PSI_KERNEL_CLASS_LINEAR);
             cuda_check(launch_linear_step(p, static_cast<uint32_t>(std::min(items, wave)), ctx->stream), "linear attention launch");
         }
         const uint64_t sms = static_cast<uint64_t>(ctx->sm_count);
-        const bool fixed = ctx->capturing;
         const auto launch_runs = [&](bool state_only, uint64_t runs) {
             const uint64_t ctas = fixed ? sms : std::min(sms, runs * l->cfg.num_v_heads);
             LaunchScope scope(ctx, PSI_KERNEL_CLASS_LINEAR);

@@ -177,6 +177,7 @@ int32_t psi_gqa_weigh_keys(psi_gqa* g, psi_pages* pages, psi_table* table, uint3
         require(g->prepared, "GQA batch metadata must be updated before recording");
         require(q != nullptr && weights != nullptr, "q and weights must not be null");
         const bool fixed = g->replay_reserved;
+        require(ctx->capturing || !stream_captured(ctx), "capture key-weight launches by psi_ctx_capture_begin: the component has to know of their graph");
         require(!ctx->capturing || fixed, "reserve replay capacity before capturing key-weight launches");
         ctx->bind();
         if (!w.planned) {
@@ -284,7 +285,7 @@ int32_t psi_gqa_evict(psi_gqa* g, psi_pages* pages, psi_table* table, uint32_t l
     if (g == nullptr) return PSI_ERR_INVALID_ARGUMENT;
     return guarded(g->ctx, [&] {
         psi_ctx* ctx = g->ctx;
-        require(!ctx->capturing, "psi_gqa_evict takes its sizes from host arrays and stays outside captured graphs");
+        require(!stream_captured(ctx), "psi_gqa_evict takes its sizes from host arrays and stays outside captured graphs");
         require(num_reqs == 0 || (src_slots != nullptr && dst_slots != nullptr && lengths != nullptr && keeps != nullptr),
                 "eviction inputs must not be null");
         require(weights != nullptr && weights_out != nullptr && kept != nullptr, "weights, weights_out and kept must not be null");
